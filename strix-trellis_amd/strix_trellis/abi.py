@@ -1,4 +1,4 @@
-"""ctypes mirror of include/strix_trellis.h and include/strix_trellis_amd.h.
+"""ctypes mirror of include/strix_trellis.h, strix_trellis_amd.h and strix_trellis_ops.h.
 
 Struct layouts follow the C header field by field (reference
 include/strix_trellis.h:57-262); enums are 32-bit.  ``load()`` opens the
@@ -14,7 +14,7 @@ TRANSPORT_VERSION = 1
 WORKSPACE_ALIGNMENT = 256
 MARKER = {"3inst": 0, "mcg": 0xCBAC1FED, "mul1": 0x83DCD12D}
 CODEBOOK = {"3inst": 0, "mcg": 1, "mul1": 2}
-DTYPE_F32 = 3
+DTYPE_F16, DTYPE_BF16, DTYPE_F32, DTYPE_I8 = 1, 2, 3, 16
 TRANSPORT_EXL3_CANONICAL = 1
 OPERATION_GEMV = 0
 OPERATION_GEMM = 1
@@ -127,6 +127,40 @@ class TpSwigluDesc(C.Structure):
                 ("diagnostic_bytes", u64), ("reserved", u64 * 4)]
 
 
+class View(C.Structure):
+    _fields_ = [("struct_size", u32), ("abi_version", u32), ("data", vp), ("buffer_bytes", u64), ("dtype", u32),
+                ("flags", u32), ("rows", u64), ("width", u64), ("row_stride", u64), ("reserved", u64 * 2)]
+
+
+class Buffer(C.Structure):
+    _fields_ = [("data", vp), ("bytes", u64)]
+
+
+class Int8WeightsDesc(C.Structure):
+    _fields_ = [("struct_size", u32), ("abi_version", u32), ("weights", View), ("scales", Buffer), ("bias", Buffer),
+                ("reserved", u64 * 4)]
+
+
+class Int8LinearDesc(C.Structure):
+    _fields_ = [("struct_size", u32), ("abi_version", u32), ("weights", vp), ("input", View),
+                ("input_scales", Buffer), ("output", View), ("alpha", f32), ("beta", f32), ("workspace", Buffer),
+                ("reserved", u64 * 4)]
+
+
+class BlockNormDesc(C.Structure):
+    _fields_ = [("struct_size", u32), ("abi_version", u32), ("block", View), ("residual", View), ("gate", View),
+                ("hidden", View), ("normed", View), ("post_weight", Buffer), ("post_bias", Buffer),
+                ("pre_weight", Buffer), ("pre_bias", Buffer), ("channel_scale", Buffer), ("norm", u32),
+                ("gate_activation", u32), ("eps", f32), ("weight_offset", f32), ("residual_scale", f32),
+                ("block_scale", f32), ("reserved", u64 * 4)]
+
+
+class TokenLogprobsDesc(C.Structure):
+    _fields_ = [("struct_size", u32), ("abi_version", u32), ("logits", View), ("tokens", Buffer),
+                ("logprobs", Buffer), ("ranks", Buffer), ("entropy", Buffer), ("top_ids", Buffer),
+                ("top_logprobs", Buffer), ("top", u32), ("scale", f32), ("workspace", Buffer), ("reserved", u64 * 4)]
+
+
 def header(struct_type, **fields):
     """Zero-initialised descriptor with struct_size / abi_version set."""
     d = struct_type()
@@ -215,6 +249,19 @@ _PROTOTYPES = {
     "strix_tp_swiglu_plan_create": (_S, [vp, C.POINTER(TpSwigluDesc), C.POINTER(Stream), C.POINTER(vp)]),
     "strix_tp_swiglu_plan_submit": (_S, [vp]),
     "strix_tp_swiglu_plan_destroy": (_S, [vp]),
+    "strix_amd_op_plan_submit": (_S, [vp]),
+    "strix_amd_op_plan_destroy": (_S, [vp]),
+    "strix_amd_int8_weights_prepare": (_S, [vp, C.POINTER(Int8WeightsDesc), C.POINTER(Stream), C.POINTER(vp)]),
+    "strix_amd_int8_weights_destroy": (_S, [vp]),
+    "strix_amd_int8_linear_workspace_bytes": (_S, [vp, C.POINTER(Int8LinearDesc), C.POINTER(u64)]),
+    "strix_amd_int8_linear": (_S, [vp, C.POINTER(Int8LinearDesc), C.POINTER(Stream)]),
+    "strix_amd_int8_linear_plan_create": (_S, [vp, C.POINTER(Int8LinearDesc), C.POINTER(Stream), C.POINTER(vp)]),
+    "strix_amd_block_norm": (_S, [vp, C.POINTER(BlockNormDesc), C.POINTER(Stream)]),
+    "strix_amd_block_norm_plan_create": (_S, [vp, C.POINTER(BlockNormDesc), C.POINTER(Stream), C.POINTER(vp)]),
+    "strix_amd_token_logprobs_workspace_bytes": (_S, [vp, C.POINTER(TokenLogprobsDesc), C.POINTER(u64)]),
+    "strix_amd_token_logprobs": (_S, [vp, C.POINTER(TokenLogprobsDesc), C.POINTER(Stream)]),
+    "strix_amd_token_logprobs_plan_create": (_S, [vp, C.POINTER(TokenLogprobsDesc), C.POINTER(Stream),
+                                                  C.POINTER(vp)]),
 }
 
 GEMV_POLL_DEFAULT = 1 << 22

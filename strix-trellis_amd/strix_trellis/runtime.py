@@ -651,3 +651,209 @@ class TpSwigluPlan:
         if self.handle:
             abi.check(self.lib.strix_tp_swiglu_plan_destroy(self.handle), "strix_tp_swiglu_plan_destroy")
             self.handle = None
+
+
+# ---------------------------------------------------------------------------
+# Operators around the trellis layers (include/strix_trellis_ops.h)
+# ---------------------------------------------------------------------------
+
+
+def _dtype_code(t):
+    """ABI element type of a torch tensor or DeviceArray, or None."""
+    name = str(t.dtype).split(".")[-1]
+    return {"float32": abi.DTYPE_F32, "float16": abi.DTYPE_F16, "bfloat16": abi.DTYPE_BF16,
+            "int8": abi.DTYPE_I8}.get(name)
+
+
+def op_view(t):
+    """strix_amd_view of a tensor [rows, width] (unit channel stride, any row stride); None: absent.
+
+    A width-1 column of a wider tensor passes as [rows, 1]."""
+    if t is None:
+        return abi.View()
+    code = _dtype_code(t)
+    if code is None or t.dim() != 2:
+        raise ValueError("rows must be float32, float16, bfloat16 or int8 tensors [rows, width]")
+    rows, width = int(t.shape[0]), int(t.shape[1])
+    stride = t.stride(0) if _is_torch(t) else width
+    if _is_torch(t) and width > 1 and t.stride(1) != 1:
+        raise ValueError("rows must have unit channel stride")
+    extent = (max(rows - 1, 0) * stride + width) * t.element_size() if rows else 0
+    return abi.header(abi.View, data=C.c_void_p(t.data_ptr() or None), buffer_bytes=extent, dtype=code, rows=rows,
+                      width=width, row_stride=stride)
+
+
+def op_buffer(t, dtype="float32"):
+    """strix_amd_buffer of a contiguous 4-byte tensor; None: absent."""
+    if t is None:
+        return abi.Buffer()
+    if str(t.dtype).split(".")[-1] != dtype or not t.is_contiguous():
+        raise ValueError(f"expected a contiguous {dtype} tensor")
+    return abi.Buffer(t.data_ptr() or None, t.numel() * 4)
+
+
+class _OpPlan:
+    """A prepared operator: `submit()` enqueues it on the stream it was created with."""
+
+    def _create(self, ctx, create, desc, stream, keep):
+        self.lib = ctx.lib
+        self._keep = keep
+        self._submit = ctx.lib.strix_amd_op_plan_submit
+        h = C.c_void_p()
+        abi.check(create(ctx.handle, C.byref(desc), C.byref(stream_desc(stream)), C.byref(h)), create.__name__)
+        self.handle = h
+
+    def submit(self):
+        status = self._submit(self.handle)
+        if status:
+            abi.check(status, "strix_amd_op_plan_submit")
+
+    def destroy(self):
+        if self.handle:
+            abi.check(self.lib.strix_amd_op_plan_destroy(self.handle), "strix_amd_op_plan_destroy")
+            self.handle = None
+
+
+def _query_workspace(ctx, query, desc):
+    need = C.c_uint64()
+    abi.check(query(ctx.handle, C.byref(desc), C.byref(need)), query.__name__)
+    return need.value
+
+
+class Int8Weights:
+    """Weights of an 8-bit integer linear layer: `w` on the device, int8 [N, I] with `scales` float32 [N], or a
+    float32, float16 or bfloat16 [N, I] that is rounded per output channel.  `bias` float32 [N] or None."""
+
+    def __init__(self, ctx, w, scales=None, bias=None, stream=None):
+        self.ctx, self.lib = ctx, ctx.lib
+        self.output, self.input = int(w.shape[0]), int(w.shape[1])
+        d = abi.header(abi.Int8WeightsDesc, weights=op_view(w), scales=op_buffer(scales), bias=op_buffer(bias))
+        h = C.c_void_p()
+        abi.check(self.lib.strix_amd_int8_weights_prepare(ctx.handle, C.byref(d), C.byref(stream_desc(stream)),
+                                                          C.byref(h)), "strix_amd_int8_weights_prepare")
+        self.handle = h
+
+    def destroy(self):
+        if self.handle:
+            abi.check(self.lib.strix_amd_int8_weights_destroy(self.handle), "strix_amd_int8_weights_destroy")
+            self.handle = None
+
+
+def _int8_desc(weights, x, y, x_scales, alpha, beta, workspace, stream):
+    d = abi.header(abi.Int8LinearDesc, weights=weights.handle, input=op_view(x), input_scales=op_buffer(x_scales),
+                   output=op_view(y), alpha=alpha, beta=beta)
+    if workspace is None:
+        need = _query_workspace(weights.ctx, weights.lib.strix_amd_int8_linear_workspace_bytes, d)
+        workspace = _on_stream(alloc_workspace(need, x.device, x), stream)
+    d.workspace = abi.Buffer(workspace.data_ptr() or None, workspace.numel() * workspace.element_size())
+    return d, workspace
+
+
+def int8_linear_workspace_bytes(weights, x, y, x_scales=None):
+    d = abi.header(abi.Int8LinearDesc, weights=weights.handle, input=op_view(x), input_scales=op_buffer(x_scales),
+                   output=op_view(y), alpha=1.0)
+    return _query_workspace(weights.ctx, weights.lib.strix_amd_int8_linear_workspace_bytes, d)
+
+
+def int8_linear(weights, x, y, x_scales=None, alpha=1.0, beta=0.0, workspace=None, stream=None):
+    """y = alpha * Int8Linear(x) + beta * y: x [rows, I] float32, float16 or bfloat16 (rounded to int8 per row), or
+    int8 with `x_scales` float32 [rows]; y [rows, N] float32, float16 or bfloat16."""
+    d, workspace = _int8_desc(weights, x, y, x_scales, alpha, beta, workspace, stream)
+    abi.check(weights.lib.strix_amd_int8_linear(weights.ctx.handle, C.byref(d), C.byref(stream_desc(stream))),
+              "strix_amd_int8_linear")
+    return y
+
+
+class Int8LinearPlan(_OpPlan):
+    """Prepared `int8_linear` on fixed buffers."""
+
+    def __init__(self, weights, x, y, x_scales=None, alpha=1.0, beta=0.0, workspace=None, stream=None):
+        d, workspace = _int8_desc(weights, x, y, x_scales, alpha, beta, workspace, stream)
+        self._create(weights.ctx, weights.lib.strix_amd_int8_linear_plan_create, d, stream,
+                     (weights, x, y, x_scales, workspace))
+
+
+NORM_KINDS = {"rms": 0, "layer": 1}
+GATE_ACTIVATIONS = {"linear": 0, "sigmoid": 1}
+
+
+def _block_norm_desc(block, residual, gate, gate_activation, hidden, normed, post_weight, post_bias, pre_weight,
+                     pre_bias, channel_scale, kind, eps, weight_offset, residual_scale, block_scale):
+    return abi.header(abi.BlockNormDesc, block=op_view(block), residual=op_view(residual), gate=op_view(gate),
+                      hidden=op_view(hidden), normed=op_view(normed), post_weight=op_buffer(post_weight),
+                      post_bias=op_buffer(post_bias), pre_weight=op_buffer(pre_weight), pre_bias=op_buffer(pre_bias),
+                      channel_scale=op_buffer(channel_scale), norm=NORM_KINDS[kind],
+                      gate_activation=GATE_ACTIVATIONS[gate_activation] if gate is not None else 0, eps=eps,
+                      weight_offset=weight_offset, residual_scale=residual_scale, block_scale=block_scale)
+
+
+def block_norm(ctx, block=None, residual=None, gate=None, gate_activation="linear", hidden=None, normed=None,
+               post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, channel_scale=None, kind="rms",
+               eps=1e-6, weight_offset=0.0, residual_scale=1.0, block_scale=1.0, stream=None):
+    """The norms and the residual sum between two blocks, in one pass:
+
+    hidden = residual_scale * residual + block_scale * channel_scale * act(gate) * norm(block; post_weight, post_bias)
+    normed = norm(hidden; pre_weight, pre_bias)
+
+    Rows [rows, width] of one type; absent parts drop out (no post_weight: the block's output as it is).  `hidden`
+    and `normed` may be the block's or the residual's own memory."""
+    d = _block_norm_desc(block, residual, gate, gate_activation, hidden, normed, post_weight, post_bias, pre_weight,
+                         pre_bias, channel_scale, kind, eps, weight_offset, residual_scale, block_scale)
+    abi.check(ctx.lib.strix_amd_block_norm(ctx.handle, C.byref(d), C.byref(stream_desc(stream))),
+              "strix_amd_block_norm")
+
+
+class BlockNormPlan(_OpPlan):
+    """Prepared `block_norm` on fixed buffers."""
+
+    def __init__(self, ctx, block=None, residual=None, gate=None, gate_activation="linear", hidden=None, normed=None,
+                 post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, channel_scale=None, kind="rms",
+                 eps=1e-6, weight_offset=0.0, residual_scale=1.0, block_scale=1.0, stream=None):
+        d = _block_norm_desc(block, residual, gate, gate_activation, hidden, normed, post_weight, post_bias,
+                             pre_weight, pre_bias, channel_scale, kind, eps, weight_offset, residual_scale,
+                             block_scale)
+        self._create(ctx, ctx.lib.strix_amd_block_norm_plan_create, d, stream,
+                     (block, residual, gate, hidden, normed, post_weight, post_bias, pre_weight, pre_bias,
+                      channel_scale))
+
+
+def _logprobs_desc(ctx, logits, tokens, logprobs, ranks, entropy, top_ids, top_logprobs, scale, workspace, stream):
+    top = 0
+    for t in (top_ids, top_logprobs):
+        if t is not None:
+            top = int(t.shape[1])
+            if t.dim() != 2 or t.shape[0] != logits.shape[0]:
+                raise ValueError("top_ids and top_logprobs must be [rows, top]")
+    if top_ids is not None and top_logprobs is not None and top_ids.shape[1] != top_logprobs.shape[1]:
+        raise ValueError("top_ids and top_logprobs must have one shape")
+    d = abi.header(abi.TokenLogprobsDesc, logits=op_view(logits), tokens=op_buffer(tokens, "int32"),
+                   logprobs=op_buffer(logprobs), ranks=op_buffer(ranks, "int32"), entropy=op_buffer(entropy),
+                   top_ids=op_buffer(top_ids, "int32"), top_logprobs=op_buffer(top_logprobs), top=top, scale=scale)
+    if workspace is None:
+        need = _query_workspace(ctx, ctx.lib.strix_amd_token_logprobs_workspace_bytes, d)
+        workspace = _on_stream(alloc_workspace(need, logits.device, logits), stream)
+    d.workspace = abi.Buffer(workspace.data_ptr() or None, workspace.numel() * workspace.element_size())
+    return d, workspace
+
+
+def token_logprobs(ctx, logits, tokens=None, logprobs=None, ranks=None, entropy=None, top_ids=None,
+                   top_logprobs=None, scale=1.0, workspace=None, stream=None):
+    """Log probabilities (nats) behind the output head, of softmax(scale * logits) per row of logits [rows, vocab]:
+    `logprobs` float32 [rows] and `ranks` int32 [rows] of `tokens` int32 [rows], `entropy` float32 [rows], and the
+    first tokens of each row, `top_ids` int32 [rows, top] and `top_logprobs` float32 [rows, top] (equal logits by
+    the lower id).  Outputs that are None are not computed."""
+    d, workspace = _logprobs_desc(ctx, logits, tokens, logprobs, ranks, entropy, top_ids, top_logprobs, scale,
+                                  workspace, stream)
+    abi.check(ctx.lib.strix_amd_token_logprobs(ctx.handle, C.byref(d), C.byref(stream_desc(stream))),
+              "strix_amd_token_logprobs")
+
+
+class TokenLogprobsPlan(_OpPlan):
+    """Prepared `token_logprobs` on fixed buffers."""
+
+    def __init__(self, ctx, logits, tokens=None, logprobs=None, ranks=None, entropy=None, top_ids=None,
+                 top_logprobs=None, scale=1.0, workspace=None, stream=None):
+        d, workspace = _logprobs_desc(ctx, logits, tokens, logprobs, ranks, entropy, top_ids, top_logprobs, scale,
+                                      workspace, stream)
+        self._create(ctx, ctx.lib.strix_amd_token_logprobs_plan_create, d, stream,
+                     (logits, tokens, logprobs, ranks, entropy, top_ids, top_logprobs, workspace))
