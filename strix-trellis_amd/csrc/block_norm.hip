@@ -26,102 +26,139 @@ __device__ __forceinline__ float group_sum(float v, float* slot) {
     return v;
 }
 
-// v -> norm(v) * (offset + weight) + bias over the row.
+// A thread's share of a row (or of a vector): groups of four channels, the
+// workgroup's groups side by side.  Every group but the last lies inside the
+// row: C is the least that covers the width.
+template <class T, int THREADS, int C>
+struct Share {
+    Raw4<T> raw[C];
+    __device__ __forceinline__ void load(const T* row, uint32_t width) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) raw[c] = load4(row, (c * THREADS + threadIdx.x) * 4, width, c + 1 < C);
+    }
+};
+
+// v -> norm(v) * (offset + weight) + bias over the row.  Channels past the
+// width are 0 before and after.  A weight that is not there yet (`late`) is
+// loaded behind the sums' inputs, so it arrives while they are added up.
 template <int THREADS, int C>
-__device__ __forceinline__ void normalise(float (&v)[C][4], const NormCall& a, const float* weight, const float* bias,
-                                          float* slots) {
+__device__ __forceinline__ void normalise(float (&v)[C][4], const NormCall& a, Share<float, THREADS, C>& weight,
+                                          const float* late, Share<float, THREADS, C>& bias, const float* with_bias,
+                                          bool late_bias, float* slots) {
     const uint32_t width = a.width;
-    float mean = 0.0f;
+    if (late) weight.load(late, width);
     if (a.layer) {
         float s = 0.0f;
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s += v[c][i];   // channels past the width are 0
-        mean = group_sum<THREADS>(s, slots) / float(width);
+            for (int i = 0; i < 4; ++i) s += v[c][i];
+        const float mean = group_sum<THREADS>(s, slots) / float(width);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t k = (c * THREADS + threadIdx.x) * 4 + i;
+                v[c][i] = c + 1 < C || k < width ? v[c][i] - mean : 0.0f;
+            }
     }
     float s = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t k = (c * THREADS + threadIdx.x) * 4 + i;
-            if (a.layer) v[c][i] = k < width ? v[c][i] - mean : 0.0f;
-            s = __builtin_fmaf(v[c][i], v[c][i], s);
-        }
+        for (int i = 0; i < 4; ++i) s = __builtin_fmaf(v[c][i], v[c][i], s);
     s = group_sum<THREADS>(s, slots + 16) / float(width);
     const float inv = 1.0f / sqrtf(s + a.eps);
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const uint32_t k = (c * THREADS + threadIdx.x) * 4;
-        if (k >= width) continue;
-        float w[4], b[4] = {};
-        load_row<4>(weight, k, width, 0.0f, w);
-        if (bias) load_row<4>(bias, k, width, 0.0f, b);
+    for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[c][i] = v[c][i] * inv * (a.weight_offset + w[i]);
-            if (bias) v[c][i] += b[i];
-        }
+        for (int i = 0; i < 4; ++i) v[c][i] = v[c][i] * inv * (a.weight_offset + weight.raw[c].v[i]);
+    if (with_bias) {
+        if (late_bias) bias.load(with_bias, width);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[c][i] += bias.raw[c].v[i];
     }
 }
 
-template <class T, int THREADS, int C>
+// A row's latency is one round trip to memory if every load is issued ahead of
+// the first sum, but the loads have to fit the registers.  kEarly: all but
+// biases and channel scales, which are loaded where they are used; kAll: those
+// too (few calls have them); kLate: rows too wide for either also load the gate
+// and the weights where they are used.
+enum Loads { kLate, kEarly, kAll };
+template <class T, int THREADS, int C, Loads LOADS>
 __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormCall a) {
     __shared__ float slots[64];
     const uint64_t row = blockIdx.x;
     const uint32_t width = a.width;
     auto at = [&](const OpRows& r) { return static_cast<const T*>(r.data) + row * r.stride; };
-    auto chan = [&](int c) { return (c * THREADS + threadIdx.x) * 4; };
-    float v[C][4], g[C][4], h[C][4];
+    Share<T, THREADS, C> block, residual, gate;
+    Share<float, THREADS, C> post, pre, post_bias, pre_bias, channel;
+    constexpr bool EARLY = LOADS != kLate, ALL = LOADS == kAll;
+    const bool full_gate = a.gate.data && !a.gate_per_row;
+    float row_gate = 1.0f;
+    if (a.block.data) block.load(at(a.block), width);
+    if (EARLY && a.post_weight) post.load(a.post_weight, width);
+    if (a.residual.data) residual.load(at(a.residual), width);
+    if (EARLY && full_gate) gate.load(at(a.gate), width);
+    if (a.gate.data && !full_gate) row_gate = float(ld_global(at(a.gate)));
+    if (EARLY && a.pre_weight) pre.load(a.pre_weight, width);
+    if (ALL && a.post_bias) post_bias.load(a.post_bias, width);
+    if (ALL && a.channel_scale) channel.load(a.channel_scale, width);
+    if (ALL && a.pre_bias) pre_bias.load(a.pre_bias, width);
+
+    float v[C][4];
     if (a.block.data) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) load_row<4>(at(a.block), chan(c), width, 0.0f, v[c]);
+        for (int c = 0; c < C; ++c) block.raw[c].to(v[c]);
+        if (a.post_weight)
+            normalise<THREADS>(v, a, post, EARLY ? nullptr : a.post_weight, post_bias, a.post_bias, !ALL, slots);
+        if (!EARLY && full_gate) gate.load(at(a.gate), width);
+        auto act = [&](float g) { return a.sigmoid ? 1.0f / (1.0f + expf(-g)) : g; };
+        if (!full_gate) row_gate = a.block_scale * (a.gate.data ? act(row_gate) : 1.0f);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float g[4];
+            if (full_gate) gate.raw[c].to(g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[c][i] *= full_gate ? a.block_scale * act(g[i]) : row_gate;
+        }
+        if (a.channel_scale) {
+            if (!ALL) channel.load(a.channel_scale, width);
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[c][i] *= channel.raw[c].v[i];
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[c][i] = 0.0f;
     }
-    // every load ahead of the first sum
     if (a.residual.data) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) load_row<4>(at(a.residual), chan(c), width, 0.0f, h[c]);
-    }
-    float row_gate = 1.0f;
-    const bool full_gate = a.gate.data && !a.gate_per_row;
-    if (full_gate) {
+        for (int c = 0; c < C; ++c) {
+            float h[4];
+            residual.raw[c].to(h);
 #pragma unroll
-        for (int c = 0; c < C; ++c) load_row<4>(at(a.gate), chan(c), width, 0.0f, g[c]);
-    } else if (a.gate.data) {
-        row_gate = float(ld_global(at(a.gate)));
-        if (a.sigmoid) row_gate = 1.0f / (1.0f + expf(-row_gate));
-    }
-    if (a.block.data && a.post_weight) normalise<THREADS>(v, a, a.post_weight, a.post_bias, slots);
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const uint32_t k = chan(c);
-        if (a.block.data) {
-            float cs[4];
-            if (a.channel_scale) load_row<4>(a.channel_scale, k, width, 0.0f, cs);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float t = v[c][i] * row_gate;
-                if (full_gate) t *= a.sigmoid ? 1.0f / (1.0f + expf(-g[c][i])) : g[c][i];
-                if (a.channel_scale) t *= cs[i];
-                v[c][i] = a.block_scale * t;
-                if (a.residual.data) v[c][i] = __builtin_fmaf(a.residual_scale, h[c][i], v[c][i]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[c][i] = a.residual_scale * h[c][i];
+            for (int i = 0; i < 4; ++i) v[c][i] = __builtin_fmaf(a.residual_scale, h[i], v[c][i]);
         }
-        if (a.hidden.data) store_row<4>(const_cast<T*>(at(a.hidden)), k, width, v[c]);
     }
+    auto store = [&](const OpRows& to) {
+        T* out = const_cast<T*>(at(to));
+#pragma unroll
+        for (int c = 0; c < C; ++c) store4(out, (c * THREADS + threadIdx.x) * 4, width, v[c]);
+    };
+    if (a.hidden.data) store(a.hidden);
     if (!a.normed.data) return;
-    // channels past the width: 0 again, whatever a gate made of them
+    // channels past the width: 0 again, whatever a gate or a bias made of them
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[c][i] = chan(c) + i < width ? v[c][i] : 0.0f;
-    normalise<THREADS>(v, a, a.pre_weight, a.pre_bias, slots + 32);
-#pragma unroll
-    for (int c = 0; c < C; ++c) store_row<4>(const_cast<T*>(at(a.normed)), chan(c), width, v[c]);
+    for (int i = 0; i < 4; ++i) v[C - 1][i] = ((C - 1) * THREADS + threadIdx.x) * 4 + i < width ? v[C - 1][i] : 0.0f;
+    normalise<THREADS>(v, a, pre, EARLY ? nullptr : a.pre_weight, pre_bias, a.pre_bias, !ALL, slots + 32);
+    store(a.normed);
 }
 
 template <class T>
@@ -131,14 +168,26 @@ hipError_t dispatch(const NormCall& a, hipStream_t stream) {
         hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, stream, a);
         return hipGetLastError();
     };
-    const uint32_t width = a.width;
-    if (width <= 256) return go(block_norm_kernel<T, 64, 1>, 64);
-    if (width <= 1024) return go(block_norm_kernel<T, 256, 1>, 256);
-    if (width <= 2048) return go(block_norm_kernel<T, 256, 2>, 256);
-    if (width <= 5120) return go(block_norm_kernel<T, 256, 5>, 256);
-    if (width <= 8192) return go(block_norm_kernel<T, 512, 4>, 512);
-    if (width <= 16384) return go(block_norm_kernel<T, 1024, 4>, 1024);
-    if (width <= 32768) return go(block_norm_kernel<T, 1024, 8>, 1024);
+    const uint32_t w = a.width;
+    const bool all = a.post_bias || a.pre_bias || a.channel_scale;
+    auto early = [&](auto threads, auto c) {
+        constexpr int THREADS = decltype(threads)::value, C = decltype(c)::value;
+        return all ? go(block_norm_kernel<T, THREADS, C, kAll>, THREADS)
+                   : go(block_norm_kernel<T, THREADS, C, kEarly>, THREADS);
+    };
+    using std::integral_constant;
+    if (w <= 256) return early(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    if (w <= 1024) return early(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+    if (w <= 2048) return early(integral_constant<int, 512>{}, integral_constant<int, 1>{});
+    if (w <= 4096) return early(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+    if (w <= 6144) return early(integral_constant<int, 512>{}, integral_constant<int, 3>{});
+    if (w <= 8192) return early(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+    if (w <= 12288) return early(integral_constant<int, 1024>{}, integral_constant<int, 3>{});
+    if (w <= 16384) return go(block_norm_kernel<T, 1024, 4, kLate>, 1024);
+    if (w <= 20480) return go(block_norm_kernel<T, 1024, 5, kLate>, 1024);
+    if (w <= 24576) return go(block_norm_kernel<T, 1024, 6, kLate>, 1024);
+    if (w <= 28672) return go(block_norm_kernel<T, 1024, 7, kLate>, 1024);
+    if (w <= 32768) return go(block_norm_kernel<T, 1024, 8, kLate>, 1024);
     return hipErrorInvalidValue;
 }
 

@@ -4,6 +4,8 @@
 // block order the prepared weights have, so that both MFMA operands are read
 // as whole 1 KiB blocks, 16 bytes per lane.  The integer sums are exact, so
 // neither the split of K nor the tile a row falls into changes a bit.
+#include <utility>
+
 #include "ops_device.hpp"
 
 namespace stx {
@@ -12,103 +14,134 @@ namespace {
 
 constexpr float kLeastScale = 0x1p-126f;
 
-// q = x / s to the nearest integer, ties to even.  The estimate x * (1 / s) is
-// off by less than 2^-16, so its nearest integer is off by one at most; r = x -
-// q s is exact in the fma (a multiple of ulp(s) / 2 below 2 s), so its
-// comparison with s / 2 decides the exact quotient's rounding.
-__device__ __forceinline__ int quotient(float x, float s, float inv) {
-    const float q0 = rintf(x * inv);
-    const float r = __builtin_fmaf(-q0, s, x), half = 0.5f * s;
-    const int q = int(q0);
-    const int up = r > half || (r == half && (q & 1)), down = r < -half || (r == -half && (q & 1));
-    return q + up - down;
+// ---- rounding of a row ----
+// s = max(RN32(most / 127), 2^-126); a row with an infinity or a NaN has most =
+// inf or NaN (the maximum passes NaN on).
+struct RowScale {
+    float s, inv, half;
+    bool fine;
+};
+__device__ __forceinline__ RowScale row_scale(float most) {
+    RowScale r;
+    r.fine = most < __builtin_inff();
+    r.s = fmaxf(most / 127.0f, kLeastScale);
+    r.inv = 1.0f / r.s;
+    r.half = 0.5f * r.s;
+    return r;
+}
+__device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+template <class T>
+__device__ __forceinline__ float most_of(float most, const Raw4<T>& x) {
+    float v[4];
+    x.to(v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = maximum(most, fabsf(v[i]));
+    return most;
 }
 
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-    return uint32_t(a & 255) | uint32_t(b & 255) << 8 | uint32_t(c & 255) << 16 | uint32_t(d) << 24;
+// Four inputs as int8 in one word.  q = x / s to the nearest integer, ties to
+// even: t = x * inv + 1.5 2^23 rounds x * inv to an integer in its low mantissa
+// bits, whose last byte is q.  inv is off by half a step, so q is the nearest
+// integer of the exact quotient unless that lies within 2^-16 of a tie: then
+// |x - q s| >= s / 2, and x - q s is exact in the fma (a multiple of ulp(s) / 2
+// below 2^24 of them, or beyond s / 2), so comparing it with s / 2 decides.
+template <class T>
+__device__ __forceinline__ uint32_t round4(const Raw4<T>& x, const RowScale& r) {
+    constexpr float kMagic = 12582912.0f;
+    float v[4], t[4], d[4];
+    x.to(v);
+    bool tie = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        t[i] = __builtin_fmaf(v[i], r.inv, kMagic);
+        d[i] = __builtin_fmaf(kMagic - t[i], r.s, v[i]);
+        tie |= fabsf(d[i]) >= r.half;
+    }
+    if (__any(tie)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool odd = __builtin_bit_cast(uint32_t, t[i]) & 1;
+            const float by = fabsf(d[i]) > r.half || (fabsf(d[i]) == r.half && odd) ? 1.0f : 0.0f;
+            t[i] += __builtin_copysignf(by, d[i]);
+        }
+    }
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = __builtin_bit_cast(uint32_t, t[i]);
+    // bytes 0 of the four words
+    const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0c);
+    return r.fine ? lo | hi : 0;
 }
+__device__ __forceinline__ uint32_t word_of(const Raw4<int8_t>& x) { return __builtin_bit_cast(uint32_t, x.v); }
 
 // ---- rows into blocks ----
-// One wave per row; a lane takes 16 consecutive inputs at a time (one 16-byte
-// piece of a block).  With ROUNDS > 0 the row stays in registers between the
-// maximum and the rounding (rows of up to 1024 ROUNDS inputs), otherwise it is
-// read twice.  Rows past the last and inputs past the width become zeros.
-template <class T, int ROUNDS>
-__global__ __launch_bounds__(256) void int8_stage_kernel(const T* x, uint64_t stride, uint64_t rows, uint32_t input,
+// One workgroup per row.  A lane takes four consecutive inputs at a time, a wave
+// 256 (one coalesced load, 16 pieces of blocks), the waves every fourth 256.
+// With HELD > 0 a wave's share stays in registers between the maximum and the
+// rounding (rows of up to 1024 HELD inputs), otherwise it is read twice.  Inputs
+// past the width become zeros; rows past the last are left as they are (they
+// meet only outputs that are not written).  Eight rows share a 128-byte line of
+// the blocks, so the 16 rows of a block go to workgroups of one XCD (workgroup i
+// runs on XCD i % 8), whose L2 puts the lines together: in row order, with a
+// piece of every line in each L2, 2048 float rows of 4096 took 16.2 us for 12.7
+// (12288 int8 rows, a layer's weights, 48 for 24).
+template <class T, int HELD>
+__global__ __launch_bounds__(256) void int8_stage_kernel(const T* x, uint64_t stride, uint32_t input,
                                                          uint32_t k_blocks, const float* given, int8_t* blocks,
-                                                         float* scales) {
-    const int lane = threadIdx.x & 63;
-    const uint64_t row = uint64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const uint32_t padded = k_blocks * 64, k0 = lane * 16;
+                                                         float* scales, uint64_t rows) {
+    __shared__ float wave_most[4];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t row = blockIdx.x / 128 * 128 + blockIdx.x % 8 * 16 + blockIdx.x / 8 % 16;
+    if (row >= rows) return;
+    const uint32_t padded = k_blocks * 64;
     int8_t* to = blocks + (row >> 4) * k_blocks * 1024 + (row & 15) * 16;
-    // the piece of inputs k .. k + 15
-    auto put = [&](uint32_t k, u32x4 v) {
-        st_global(reinterpret_cast<u32x4*>(to + uint64_t(k >> 6) * 1024 + ((k >> 4) & 3) * 256), v);
-    };
-    if (row >= rows) {
-        for (uint32_t k = k0; k < padded; k += 1024) put(k, u32x4{});
-        return;
-    }
+    constexpr int kAtOnce = HELD ? HELD : 5;   // loads in flight
     const T* from = x + row * stride;
+    // inputs c .. c + 255 of the wave: every 1024; the last may reach past the end
+    const uint32_t c0 = w * 256, inside = input / 256 * 256;
+    const bool at_end = input > inside && (inside - c0) % 1024 == 0 && inside >= c0;
+    auto put = [&](uint32_t c, uint32_t q) {
+        const uint32_t k = c + lane * 4;
+        if (k < padded)
+            st_global(reinterpret_cast<uint32_t*>(to + uint64_t(k >> 6) * 1024 + ((k >> 4) & 3) * 256 + (k & 12)), q);
+    };
+    Raw4<T> raw[kAtOnce], end;
+    auto load_some = [&](uint32_t c) {
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j)
+            if (c + j * 1024 < inside) raw[j] = load4(from, c + j * 1024 + lane * 4, input, true);
+    };
+    if (at_end) end = load4(from, inside + lane * 4, input, false);
     if constexpr (std::is_same_v<T, int8_t>) {
-        for (uint32_t k = k0; k < padded; k += 1024) {
-            u32x4 v{};
-            if (k + 16 <= input) {
-                v = __builtin_bit_cast(u32x4, ld_packed<16>(from + k));
-            } else {
+        for (uint32_t c = c0; c < inside; c += kAtOnce * 1024) {
+            load_some(c);
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (k + i < input) v[i / 4] |= uint32_t(uint8_t(ld_global(from + k + i))) << (8 * (i & 3));
-            }
-            put(k, v);
+            for (int j = 0; j < kAtOnce; ++j)
+                if (c + j * 1024 < inside) put(c + j * 1024, word_of(raw[j]));
         }
-        if (given && lane == 0) st_global(scales + row, ld_global(given + row));
+        if (at_end) put(inside, word_of(end));
+        if (given && threadIdx.x == 0) st_global(scales + row, ld_global(given + row));
     } else {
-        constexpr int R = ROUNDS ? ROUNDS : 1;
-        float v[R][16];
-        float most = 0.0f, bad = 0.0f;   // bad: 0, or NaN once an infinity or a NaN was seen
-        auto look = [&](const float (&u)[16]) {
+        float most = 0.0f;
+        for (uint32_t c = c0; c < inside; c += kAtOnce * 1024) {
+            load_some(c);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                most = fmaxf(most, fabsf(u[i]));
-                bad += u[i] * 0.0f;
-            }
-        };
-        if constexpr (ROUNDS > 0) {
-#pragma unroll
-            for (int c = 0; c < R; ++c) load_row<16>(from, k0 + c * 1024, input, 0.0f, v[c]);
-#pragma unroll
-            for (int c = 0; c < R; ++c) look(v[c]);
-        } else {
-            for (uint32_t k = k0; k < input; k += 1024) {
-                load_row<16>(from, k, input, 0.0f, v[0]);
-                look(v[0]);
-            }
+            for (int j = 0; j < kAtOnce; ++j)
+                if (c + j * 1024 < inside) most = most_of(most, raw[j]);
         }
-        most = wave_max(most);
-        bad = wave_sum(bad);
-        const bool fine = bad == 0.0f;
-        float s = fmaxf(most / 127.0f, kLeastScale);
-        const float inv = 1.0f / s;
-        auto round16 = [&](const float (&u)[16]) {
-            u32x4 q;
+        if (at_end) most = most_of(most, end);
+        most = wave_reduce(most, maximum);
+        if (lane == 0) wave_most[w] = most;
+        __syncthreads();
+        const RowScale r = row_scale(maximum(maximum(wave_most[0], wave_most[1]), maximum(wave_most[2], wave_most[3])));
+        for (uint32_t c = c0; c < inside; c += kAtOnce * 1024) {
+            if (!HELD) load_some(c);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                q[j] = pack4(quotient(u[4 * j], s, inv), quotient(u[4 * j + 1], s, inv),
-                             quotient(u[4 * j + 2], s, inv), quotient(u[4 * j + 3], s, inv));
-            return fine ? q : u32x4{};
-        };
-        if constexpr (ROUNDS > 0) {
-#pragma unroll
-            for (int c = 0; c < R; ++c)
-                if (k0 + c * 1024 < padded) put(k0 + c * 1024, round16(v[c]));
-        } else {
-            for (uint32_t k = k0; k < padded; k += 1024) {
-                load_row<16>(from, k, input, 0.0f, v[0]);
-                put(k, round16(v[0]));
-            }
+            for (int j = 0; j < kAtOnce; ++j)
+                if (c + j * 1024 < inside) put(c + j * 1024, round4(raw[j], r));
         }
-        if (lane == 0) st_global(scales + row, fine ? s : __builtin_nanf(""));
+        if (at_end) put(inside, round4(end, r));
+        if (threadIdx.x == 0) st_global(scales + row, r.fine ? r.s : __builtin_nanf(""));
     }
 }
 
@@ -122,6 +155,7 @@ struct Int8Args {
     uint32_t y_type;
     uint32_t rows, output, k_blocks;
     float alpha, beta;
+    uint32_t n_tiles, m_tiles;
 };
 
 // Channels n .. n + 3 of row m from their integer sums.  Channels past the
@@ -143,7 +177,7 @@ __device__ __forceinline__ void emit4(const Int8Args& a, uint32_t m, uint32_t n,
                                       const Channels& c) {
     T* row = static_cast<T*>(a.y) + uint64_t(m) * a.y_stride;
     float v[4], old[4];
-    if (a.beta != 0.0f) load_row<4>(row, n, a.output, 0.0f, old);
+    if (a.beta != 0.0f) load4(static_cast<const T*>(row), n, a.output, false).to(old);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         v[i] = float(acc[i]) * s * c.t[i];
@@ -151,7 +185,7 @@ __device__ __forceinline__ void emit4(const Int8Args& a, uint32_t m, uint32_t n,
         v[i] *= a.alpha;
         if (a.beta != 0.0f) v[i] += a.beta * old[i];
     }
-    store_row<4>(row, n, a.output, v);
+    store4(row, n, a.output, v);
 }
 __device__ __forceinline__ void emit(const Int8Args& a, uint32_t m, uint32_t n, i32x4 acc, float s,
                                      const Channels& c) {
@@ -160,8 +194,123 @@ __device__ __forceinline__ void emit(const Int8Args& a, uint32_t m, uint32_t n, 
     else emit4<_Float16>(a, m, n, acc, s, c);
 }
 
-// Few rows (1..16): one workgroup per 16 channels, its eight waves split K and
-// add their sums in LDS.
+// ---- a few rows ----
+// One launch: every workgroup rounds the rows itself, into LDS, while its
+// weights (16 channels) are on their way.  Eight waves; the waves split K and add
+// their sums in LDS.  M: rows, rounded up to a power of two; 8 / M waves round one
+// row.  A row's share of a lane stays in registers where it fits, else it is
+// read twice (from the caches).
+template <class T, int M>
+__global__ __launch_bounds__(512, 4) void int8_decode_kernel(Int8Args a, const T* x, uint64_t stride, uint32_t input) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int G = 8 / M;                  // waves per row
+    __shared__ i32x4 part[8][64];
+    __shared__ float wave_most[8], row_s[8];
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t kbs = a.k_blocks, kb0 = kbs * w / 8, kb1 = kbs * (w + 1) / 8;
+    const uint32_t pitch = kbs * 64 + 64;     // bytes of a row in LDS: rows 16 banks apart
+    constexpr int U = 10;
+    u32x4 f[U];
+    const auto wr = make_rsrc(a.w + uint64_t(blockIdx.x) * kbs * 1024, kb1 * 1024);
+    // blocks kb .. kb + U - 1; past the wave's part they read zeros
+    auto load_w = [&](uint32_t kb) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            f[u] = __builtin_amdgcn_raw_buffer_load_b128(wr, (kb + u) * 1024 + lane * 16, 0, 0);
+    };
+
+    // ---- rows into LDS ----
+    {
+        const int m = w / G, part_of = w % G;
+        const bool live = uint32_t(m) < a.rows;
+        const T* from = x + (live ? m : 0) * stride;
+        const uint32_t padded = kbs * 64, step = G * 256;
+        unsigned char* to = smem + m * pitch;
+        auto put = [&](uint32_t b, uint32_t q) {
+            if (b + lane * 4 < padded) *reinterpret_cast<uint32_t*>(to + b + lane * 4) = q;
+        };
+        // the wave's groups of 256 inputs: b0, b0 + step, ..; the last may reach past the end
+        const uint32_t b0 = part_of * 256, inside = input / 256 * 256;
+        const bool at_end = input > inside && inside >= b0 && (inside - b0) % step == 0;
+        constexpr int kHeld = M == 1 ? 4 : M == 2 ? 6 : M == 4 ? 10 : 6;
+        Raw4<T> raw[kHeld], end;
+        auto load_some = [&](uint32_t b) {
+#pragma unroll
+            for (int c = 0; c < kHeld; ++c)
+                if (b + c * step < inside) raw[c] = load4(from, b + c * step + lane * 4, input, true);
+        };
+        // the weights behind the row: loads arrive in order, and the row's come first
+        load_some(b0);
+        if (at_end) end = load4(from, inside + lane * 4, input, false);
+        __builtin_amdgcn_sched_barrier(0);
+        load_w(kb0);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (std::is_same_v<T, int8_t>) {
+            for (uint32_t b = b0; b < inside && live; b += kHeld * step) {
+                if (b != b0) load_some(b);
+#pragma unroll
+                for (int c = 0; c < kHeld; ++c)
+                    if (b + c * step < inside) put(b + c * step, word_of(raw[c]));
+            }
+            if (at_end && live) put(inside, word_of(end));
+            if (live && lane == 0 && part_of == 0) row_s[m] = ld_global(a.s + m);
+        } else {
+            float most = 0.0f;
+            const bool held = inside <= kHeld * step;
+            for (uint32_t b = b0; b < inside; b += kHeld * step) {
+                if (b != b0) load_some(b);
+#pragma unroll
+                for (int c = 0; c < kHeld; ++c)
+                    if (b + c * step < inside) most = most_of(most, raw[c]);
+            }
+            if (at_end) most = most_of(most, end);
+            most = wave_reduce(most, maximum);
+            if constexpr (G > 1) {
+                if (lane == 0) wave_most[w] = most;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < G; ++i) most = maximum(most, wave_most[m * G + i]);
+            }
+            const RowScale r = row_scale(most);
+            for (uint32_t b = b0; b < inside && live; b += kHeld * step) {
+                if (!held) load_some(b);
+#pragma unroll
+                for (int c = 0; c < kHeld; ++c)
+                    if (b + c * step < inside) put(b + c * step, round4(raw[c], r));
+            }
+            if (at_end && live) put(inside, round4(end, r));
+            if (live && lane == 0 && part_of == 0) row_s[m] = r.fine ? r.s : __builtin_nanf("");
+        }
+    }
+    __syncthreads();
+
+    // ---- products ----
+    const uint32_t m = lane & 15, n = blockIdx.x * 16 + 4 * (lane >> 4);
+    const unsigned char* xr = smem + (m < a.rows ? m : 0) * pitch + (lane >> 4) * 16;   // dead columns repeat row 0
+    i32x4 acc{};
+    for (uint32_t kb = kb0;;) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            // past the wave's part the weights are zeros, whatever lies in LDS
+            const uint32_t at = kb + u < kbs ? kb + u : kbs - 1;
+            const i32x4 q = *reinterpret_cast<const i32x4*>(xr + at * 64);
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, f[u]), q, acc, 0, 0, 0);
+        }
+        kb += U;
+        if (kb >= kb1) break;
+        load_w(kb);
+    }
+    part[w][lane] = acc;
+    __syncthreads();
+    if (w || m >= a.rows || n >= a.output) return;
+#pragma unroll
+    for (int j = 1; j < 8; ++j) acc += part[j][lane];
+    emit(a, m, n, acc, row_s[m], channels_of(a, n));
+}
+
+// ---- nine to sixteen rows ----
+// One workgroup per 16 channels; its eight waves split K and add their sums in
+// LDS.
 __global__ __launch_bounds__(512) void int8_rows16_kernel(Int8Args a) {
     __shared__ i32x4 part[8][64];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -189,73 +338,229 @@ __global__ __launch_bounds__(512) void int8_rows16_kernel(Int8Args a) {
 #pragma unroll
     for (int j = 1; j < 8; ++j) acc += part[j][lane];
     const uint32_t m = lane & 15, n = blockIdx.x * 16 + 4 * (lane >> 4);
-    if (m < a.rows) emit(a, m, n, acc, ld_global(a.s + m), channels_of(a, n));
+    if (m < a.rows && n < a.output) emit(a, m, n, acc, ld_global(a.s + m), channels_of(a, n));
 }
 
-// Tiles of 128 channels x 128 rows, four waves of 64 x 64, both operands in a
-// ring of LDS stages of 64 inputs.
-__global__ __launch_bounds__(256) void int8_tile_kernel(Int8Args a, uint32_t n_tiles) {
-    constexpr int kStage = 16384, kRing = 4;
-    __shared__ __align__(16) unsigned char ring[kRing * kStage];
+// ---- tens to hundreds of rows ----
+// Tiles of 32 TN channels x 32 TM rows, few and short: the tile's K is split over
+// the workgroup's eight waves, each of which multiplies the whole tile over its
+// part with operands straight from the caches (both are in MFMA order, 1 KiB per
+// load), two batches of U blocks in flight and no barrier.  The sums meet in
+// LDS, [wave][row][channel] with 16-byte units at unit ^ row, and leave as whole
+// rows of the tile.
+template <int TN, int TM>
+__global__ __launch_bounds__(512, 2) void int8_direct_kernel(Int8Args a) {
+    constexpr int BN = 32 * TN, BM = 32 * TM, U = TN * TM == 1 ? 4 : TN * TM == 2 ? 3 : 2;
+    constexpr int kUnits = BN / 4, kPlane = BM * BN * 4;
+    extern __shared__ __align__(16) unsigned char smem[];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const uint32_t nt = blockIdx.x % n_tiles, mt = blockIdx.x / n_tiles;
-    const uint32_t nb = (a.output + 31) / 32 * 2, mb = (a.rows + 31) / 32 * 2, kbs = a.k_blocks;
-    const uint32_t nb0 = nt * 8, mb0 = mt * 8;
-    const uint32_t nbn = nb - nb0 < 8 ? nb - nb0 : 8, mbn = mb - mb0 < 8 ? mb - mb0 : 8;
-    const auto wr = make_rsrc(a.w + uint64_t(nb0) * kbs * 1024, nbn * kbs * 1024);
-    const auto xr = make_rsrc(a.x + uint64_t(mb0) * kbs * 1024, mbn * kbs * 1024);
-    const uint32_t pair = kbs * 1024;
-    auto dma = [&](uint32_t kb) {
-        unsigned char* base = ring + (kb % kRing) * kStage + 2 * w * 1024;
-        const uint32_t off = (kb < kbs ? kb * 1024 + lane * 16 : 0x80000000u);
+    const uint32_t nt = blockIdx.x % a.n_tiles, mt = blockIdx.x / a.n_tiles;
+    const uint32_t kbs = a.k_blocks, kb0 = kbs * w / 8, kb1 = kbs * (w + 1) / 8, pair = kbs * 1024;
+    const uint32_t nb = (a.output + 31) / 32 * 2 - nt * 2 * TN, mb = (a.rows + 31) / 32 * 2 - mt * 2 * TM;
+    // blocks of channels or rows past the last read zeros
+    const auto wr = make_rsrc(a.w + uint64_t(nt) * 2 * TN * pair, (nb < 2 * TN ? nb : 2 * TN) * pair);
+    const auto xr = make_rsrc(a.x + uint64_t(mt) * 2 * TM * pair, (mb < 2 * TM ? mb : 2 * TM) * pair);
+    const int h = lane >> 5, r16 = lane & 15, hi = (lane >> 4) & 1;
+    const uint32_t piece = hi * pair + (h * 16 + r16) * 16;
+    struct Operands {
+        u32x4 f[U][2][TN], g[U][2][TM];
+    };
+    auto load = [&](Operands& o, uint32_t kb) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void*)(base + j * 1024), 16,
-                                                     off + (2 * w + j) * pair, 0, 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                xr, (__attribute__((address_space(3))) void*)(base + 8192 + j * 1024), 16, off + (2 * w + j) * pair, 0, 0,
-                0);
+        for (int u = 0; u < U; ++u) {
+            const bool live = kb + u < kb1;   // past the wave's part: out of range, zeros
+            const uint32_t at = piece + (live ? (kb + u) * 1024 : 0x80000000u);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int i = 0; i < TN; ++i)
+                    o.f[u][j][i] = __builtin_amdgcn_raw_buffer_load_b128(wr, at + 2 * i * pair + j * 512, 0, 0);
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+                    o.g[u][j][i] = __builtin_amdgcn_raw_buffer_load_b128(xr, at + 2 * i * pair + j * 512, 0, 0);
+            }
         }
     };
-    const int wn = w & 1, wm = w >> 1, h = lane >> 5, r16 = lane & 15, hi = (lane >> 4) & 1;
-    i32x16 acc[2][2] = {};
-    dma(0);
-    dma(1);
-    dma(2);
-    for (uint32_t kb = 0; kb < kbs; ++kb) {
-        asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        dma(kb + 3);
-        const unsigned char* st = ring + (kb % kRing) * kStage;
+    i32x16 acc[TN][TM] = {};
+    auto multiply = [&](const Operands& o) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            i32x4 f[2], g[2];
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                f[i] = *reinterpret_cast<const i32x4*>(st + (wn * 4 + i * 2 + hi) * 1024 + ((2 * j + h) * 16 + r16) * 16);
-                g[i] = *reinterpret_cast<const i32x4*>(st + 8192 + (wm * 4 + i * 2 + hi) * 1024 +
-                                                       ((2 * j + h) * 16 + r16) * 16);
-            }
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < TN; ++i)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) acc[i][k] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[i], g[k], acc[i][k], 0, 0, 0);
-        }
+                    for (int k = 0; k < TM; ++k)
+                        acc[i][k] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, o.f[u][j][i]),
+                                                                          __builtin_bit_cast(i32x4, o.g[u][j][k]),
+                                                                          acc[i][k], 0, 0, 0);
+    };
+    Operands o[2];
+    load(o[0], kb0);
+    for (uint32_t kb = kb0; kb < kb1; kb += 2 * U) {
+        // the next batch's loads stay ahead of this one's products
+        load(o[1], kb + U);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(o[0]);
+        __builtin_amdgcn_sched_barrier(0);
+        load(o[0], kb + 2 * U);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(o[1]);
+        __builtin_amdgcn_sched_barrier(0);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    auto place = [&](int row, int unit) { return row * (BN * 4) + ((unit ^ row) & (kUnits - 1)) * 16; };
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const uint32_t m = mt * 128 + wm * 64 + k * 32 + (lane & 31);
-        if (m >= a.rows) continue;
-        const float s = ld_global(a.s + m);
+    for (int i = 0; i < TN; ++i)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int k = 0; k < TM; ++k)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint32_t n = nt * 128 + wn * 64 + i * 32 + 8 * q + 4 * h;
-                if (n < a.output)
-                    emit(a, m, n, i32x4{acc[i][k][4 * q], acc[i][k][4 * q + 1], acc[i][k][4 * q + 2], acc[i][k][4 * q + 3]}, s,
-                         channels_of(a, n));
-            }
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<i32x4*>(smem + w * kPlane + place(k * 32 + (lane & 31), i * 8 + 2 * q + h)) =
+                    i32x4{acc[i][k][4 * q], acc[i][k][4 * q + 1], acc[i][k][4 * q + 2], acc[i][k][4 * q + 3]};
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < (BM * kUnits + 511) / 512; ++c) {
+        const int item = c * 512 + threadIdx.x, row = item / kUnits, unit = item % kUnits;
+        const uint32_t m = mt * BM + row, n = nt * BN + unit * 4;
+        if (row >= BM || m >= a.rows || n >= a.output) continue;
+        i32x4 sum{};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += *reinterpret_cast<const i32x4*>(smem + j * kPlane + place(row, unit));
+        emit(a, m, n, sum, ld_global(a.s + m), channels_of(a, n));
+    }
+}
+
+// ---- many rows ----
+// Tiles of 64 TN channels x 64 TM rows, four waves (two along each side) of 32 TN x
+// 32 TM, both operands in a ring of LDS stages of 64 inputs that the DMA fills
+// kRing - 1 stages ahead.  A stage is two K32 steps; the fragments of a step are
+// read while the step before multiplies.  The barrier stands between a stage's
+// steps: behind it every wave has read the whole stage, so its buffer takes the
+// DMA of the stage kRing ahead, and the next stage has landed.
+template <int TN, int TM, int RING>
+struct WideShape {
+    static constexpr int kBN = 64 * TN, kBM = 64 * TM, kStage = (TN + TM) * 4096, kRing = RING;
+    static constexpr size_t kLds = size_t(kRing) * kStage;
+    static_assert(kLds >= 4u * (32 * 128 * TN + 128), "the epilogue's turn");
+};
+
+template <int TN, int TM, int RING>
+__global__ __launch_bounds__(256, 2) void int8_wide_kernel(Int8Args a) {
+    using S = WideShape<TN, TM, RING>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    // XCD-aware order: workgroup i runs on XCD i % 8, which takes a contiguous run of
+    // tiles, rows first in bands of up to eight row tiles, so its workgroups share
+    // both operands in its L2.
+    const uint32_t tiles = a.n_tiles * a.m_tiles, per = tiles / 8;
+    uint32_t t = blockIdx.x;
+    if (t < per * 8) t = (t % 8) * per + t / 8;
+    const uint32_t band = t / (8 * a.n_tiles), in_band = t - band * 8 * a.n_tiles;
+    const uint32_t height = a.m_tiles - band * 8 < 8 ? a.m_tiles - band * 8 : 8;
+    const uint32_t mt = band * 8 + in_band % height, nt = in_band / height;
+    const uint32_t kbs = a.k_blocks, pair = kbs * 1024;
+    const uint32_t nb = (a.output + 31) / 32 * 2 - nt * 4 * TN, mb = (a.rows + 31) / 32 * 2 - mt * 4 * TM;
+    // blocks of channels or rows past the last read zeros
+    const auto wr = make_rsrc(a.w + uint64_t(nt) * 4 * TN * pair, (nb < 4 * TN ? nb : 4 * TN) * pair);
+    const auto xr = make_rsrc(a.x + uint64_t(mt) * 4 * TM * pair, (mb < 4 * TM ? mb : 4 * TM) * pair);
+    // a stage: 4 TN blocks of channels, 4 TM of rows; wave w moves blocks w, w + 4, ..
+    const uint32_t lane_off = lane * 16 + w * pair;
+    auto dma = [&](uint32_t kb, uint32_t slot) {
+        unsigned char* base = smem + slot * S::kStage + w * 1024;
+        const uint32_t off = lane_off + (kb < kbs ? kb * 1024 : 0x80000000u);   // past the end: out of range
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void*)(base + j * 4096), 16,
+                                                     off + j * 4 * pair, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                xr, (__attribute__((address_space(3))) void*)(base + (TN + j) * 4096), 16, off + j * 4 * pair, 0, 0, 0);
+    };
+    const int wn = w & 1, wm = w >> 1, h = lane >> 5, r16 = lane & 15, hi = (lane >> 4) & 1;
+    const uint32_t piece = hi * 1024 + (h * 16 + r16) * 16;
+    i32x4 f[2][TN], g[2][TM];
+    auto read = [&](uint32_t slot, int j) {
+        const unsigned char* st = smem + slot * S::kStage + piece + j * 512;
+#pragma unroll
+        for (int i = 0; i < TN; ++i) f[j][i] = *reinterpret_cast<const i32x4*>(st + (wn * 2 * TN + i * 2) * 1024);
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+            g[j][i] = *reinterpret_cast<const i32x4*>(st + (4 * TN + wm * 2 * TM + i * 2) * 1024);
+    };
+    i32x16 acc[TN][TM] = {};
+    auto multiply = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int k = 0; k < TM; ++k) acc[i][k] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[j][i], g[j][k], acc[i][k], 0, 0, 0);
+        // the reads behind the first MFMAs (0x008: MFMA, 0x100: LDS read)
+        constexpr int kReads = TN + TM, kEach = TN * TM >= kReads ? 1 : 2;
+#pragma unroll
+        for (int i = 0; i < kReads / kEach; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, TN * TM - kReads / kEach, 0);
+    };
+    constexpr int kLoads = TN + TM;
+#pragma unroll
+    for (int i = 0; i < RING; ++i) dma(i, i);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((RING - 1) * kLoads) : "memory");
+    read(0, 0);
+    for (uint32_t kb = 0, slot = 0; kb < kbs; ++kb) {
+        const uint32_t ahead = slot + 1 == RING ? 0 : slot + 1;
+        __builtin_amdgcn_sched_barrier(0);
+        read(slot, 1);
+        multiply(0);
+        __builtin_amdgcn_sched_barrier(0);
+        // all but the next stage's DMAs may still be on their way
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * kLoads) : "memory");
+        dma(kb + RING, slot);
+        __builtin_amdgcn_sched_barrier(0);
+        read(ahead, 0);   // past the last stage: zeros of the DMA, not used
+        multiply(1);
+        slot = ahead;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+
+    // A lane holds four consecutive channels of 32 rows here and there; each 32-row
+    // block of a wave turns around in the wave's own part of LDS (16-byte unit u
+    // of row r at unit u ^ r), after which a store covers whole rows of the
+    // block (512 contiguous bytes of two rows at TN = 4).  A wave's LDS operations
+    // are in order: no barrier.  The row loop stays a loop: written out for every
+    // type and edge the epilogue took 95 KB of code, more than the instruction
+    // cache holds.
+    constexpr int kUnits = 8 * TN, kRowsAtOnce = 64 / kUnits, kTurn = 32 * kUnits * 16;
+    unsigned char* turn = smem + w * (kTurn + 128);
+    float* row_s = reinterpret_cast<float*>(turn + kTurn);
+    const uint32_t unit = lane % kUnits, sub = lane / kUnits;
+    const uint32_t n = nt * S::kBN + wn * 32 * TN + unit * 4, m_wave = mt * S::kBM + wm * 32 * TM;
+    const bool inside = n < a.output;
+    const Channels c = channels_of(a, inside ? n : 0);
+    float s[TM];
+#pragma unroll
+    for (int k = 0; k < TM; ++k) {
+        const uint32_t m = m_wave + k * 32 + (lane & 31);
+        s[k] = ld_global(a.s + (m < a.rows ? m : 0));
+    }
+#pragma unroll
+    for (int k = 0; k < TM; ++k) {
+        if (lane < 32) row_s[lane] = s[k];
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<i32x4*>(turn + (lane & 31) * (kUnits * 16) +
+                                          (((i * 8 + 2 * q + h) ^ lane) & (kUnits - 1)) * 16) =
+                    i32x4{acc[i][k][4 * q], acc[i][k][4 * q + 1], acc[i][k][4 * q + 2], acc[i][k][4 * q + 3]};
+#pragma unroll 4
+        for (uint32_t row = sub; row < 32; row += kRowsAtOnce) {
+            const uint32_t m = m_wave + k * 32 + row;
+            const i32x4 v = *reinterpret_cast<const i32x4*>(turn + row * (kUnits * 16) + ((unit ^ row) & (kUnits - 1)) * 16);
+            if (m < a.rows && inside) emit(a, m, n, v, row_s[row], c);
+        }
     }
 }
 
@@ -267,15 +572,98 @@ __global__ __launch_bounds__(256) void copy_f32_kernel(const float* from, float*
 template <class T>
 void stage(const OpRows& x, uint64_t rows, uint32_t input, const float* given, int8_t* blocks, float* scales,
            hipStream_t stream) {
-    const dim3 grid(uint32_t(int8_row_blocks(rows) * 4)), block(256);
+    const dim3 grid{uint32_t((rows + 127) / 128 * 128)}, block(256);
     const uint32_t kb = int8_k_blocks(input);
     const T* from = static_cast<const T*>(x.data);
-    if (input <= 5120)
-        hipLaunchKernelGGL((int8_stage_kernel<T, 5>), grid, block, 0, stream, from, x.stride, rows, input, kb, given,
-                           blocks, scales);
-    else
-        hipLaunchKernelGGL((int8_stage_kernel<T, 0>), grid, block, 0, stream, from, x.stride, rows, input, kb, given,
-                           blocks, scales);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, block, 0, stream, from, x.stride, input, kb, given, blocks, scales, rows);
+    };
+    if (input <= 5 * 1024) go(int8_stage_kernel<T, 5>);
+    else if (input <= 8 * 1024) go(int8_stage_kernel<T, 8>);
+    else go(int8_stage_kernel<T, 0>);
+}
+
+template <class T>
+hipError_t decode(const Int8Args& a, const OpRows& x, uint32_t input, hipStream_t stream) {
+    const size_t lds = size_t(a.rows) * (a.k_blocks * 64 + 64);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((a.output + 15) / 16), dim3(512), lds, stream, a,
+                           static_cast<const T*>(x.data), x.stride, input);
+        return hipGetLastError();
+    };
+    if (a.rows <= 1) return go(int8_decode_kernel<T, 1>);
+    if (a.rows <= 2) return go(int8_decode_kernel<T, 2>);
+    if (a.rows <= 4) return go(int8_decode_kernel<T, 4>);
+    return go(int8_decode_kernel<T, 8>);
+}
+
+template <class F>
+hipError_t launch_core(F kernel, uint32_t tiles, uint32_t threads, size_t lds, const Int8Args& a, hipStream_t stream) {
+    hipLaunchKernelGGL(kernel, dim3(tiles), dim3(threads), lds, stream, a);
+    return hipGetLastError();
+}
+
+using Wide256x128 = WideShape<4, 2, 3>;
+using Wide128x128 = WideShape<2, 2, 3>;
+
+// Kernels with more than 64 KiB of LDS have to be told, once.
+hipError_t allow_lds() {
+    static const hipError_t status = [] {
+        const std::pair<void (*)(Int8Args), size_t> large[] = {{int8_direct_kernel<2, 2>, 8 * 16384},
+                                                               {int8_wide_kernel<4, 2, 3>, Wide256x128::kLds}};
+        for (const auto& [kernel, lds] : large) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
+            if (e != hipSuccess) return e;
+        }
+        return hipSuccess;
+    }();
+    return status;
+}
+
+hipError_t launch_pass(const Int8Layer& w, const Int8Call& call, hipStream_t stream) {
+    const Int8Plan plan = int8_plan(call.rows, w.input, w.output);
+    auto* blocks = static_cast<int8_t*>(call.workspace);
+    Int8Args a{};
+    a.w = w.blocks;
+    a.x = blocks;
+    a.t = w.scales;
+    a.bias = w.bias;
+    a.y = const_cast<void*>(call.y.data);
+    a.y_stride = call.y.stride;
+    a.y_type = call.y.type;
+    a.rows = uint32_t(call.rows);
+    a.output = w.output;
+    a.k_blocks = int8_k_blocks(w.input);
+    a.alpha = call.alpha;
+    a.beta = call.beta;
+    a.n_tiles = plan.n_tiles;
+    a.m_tiles = plan.m_tiles;
+    if (plan.core == kInt8Decode) {
+        a.s = call.x_scales;
+        switch (call.x.type) {
+            case kF32: return decode<float>(a, call.x, w.input, stream);
+            case kF16: return decode<_Float16>(a, call.x, w.input, stream);
+            case kBF16: return decode<__bf16>(a, call.x, w.input, stream);
+            case kI8: return decode<int8_t>(a, call.x, w.input, stream);
+            default: return hipErrorInvalidValue;
+        }
+    }
+    auto* scales = reinterpret_cast<float*>(blocks + plan.scales_at);
+    a.s = scales;
+    hipError_t e = allow_lds();
+    if (e == hipSuccess) e = launch_int8_stage(call.x, call.rows, w.input, call.x_scales, blocks, scales, stream);
+    if (e != hipSuccess) return e;
+    const uint32_t tiles = plan.n_tiles * plan.m_tiles;
+    switch (plan.core) {
+        case kInt8Rows16: return launch_core(int8_rows16_kernel, tiles, 512, 0, a, stream);
+        case kInt8Direct32x32: return launch_core(int8_direct_kernel<1, 1>, tiles, 512, 8 * 4096, a, stream);
+        case kInt8Direct32x64: return launch_core(int8_direct_kernel<1, 2>, tiles, 512, 8 * 8192, a, stream);
+        case kInt8Direct64x64: return launch_core(int8_direct_kernel<2, 2>, tiles, 512, 8 * 16384, a, stream);
+        case kInt8Wide256x128: return launch_core(int8_wide_kernel<4, 2, 3>, tiles, 256, Wide256x128::kLds, a, stream);
+        case kInt8Wide128x128: return launch_core(int8_wide_kernel<2, 2, 3>, tiles, 256, Wide128x128::kLds, a, stream);
+        default: return hipErrorInvalidValue;
+    }
 }
 
 }  // namespace
@@ -287,43 +675,26 @@ hipError_t launch_copy_f32(const float* from, float* to, uint64_t count, hipStre
 
 hipError_t launch_int8_stage(const OpRows& x, uint64_t rows, uint32_t input, const float* given, int8_t* blocks,
                              float* scales, hipStream_t stream) {
-    switch (x.type) {
-        case kF32: stage<float>(x, rows, input, given, blocks, scales, stream); break;
-        case kF16: stage<_Float16>(x, rows, input, given, blocks, scales, stream); break;
-        case kBF16: stage<__bf16>(x, rows, input, given, blocks, scales, stream); break;
-        case kI8: stage<int8_t>(x, rows, input, given, blocks, scales, stream); break;
-        default: return hipErrorInvalidValue;
+    constexpr uint64_t kRows = 1u << 20;   // a launch holds fewer than 2^32 threads
+    OpRows part = x;
+    for (uint64_t left = rows; left;) {
+        const uint64_t n = left < kRows ? left : kRows;
+        switch (x.type) {
+            case kF32: stage<float>(part, n, input, given, blocks, scales, stream); break;
+            case kF16: stage<_Float16>(part, n, input, given, blocks, scales, stream); break;
+            case kBF16: stage<__bf16>(part, n, input, given, blocks, scales, stream); break;
+            case kI8: stage<int8_t>(part, n, input, given, blocks, scales, stream); break;
+            default: return hipErrorInvalidValue;
+        }
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        left -= n;
+        part.data = static_cast<const char*>(part.data) + n * x.stride * (x.type == kF32 ? 4 : x.type == kI8 ? 1 : 2);
+        if (given) given += n;
+        blocks += n / 16 * int8_k_blocks(input) * 1024;
+        scales += n;
     }
-    return hipGetLastError();
-}
-
-static hipError_t launch_pass(const Int8Layer& w, const Int8Call& call, hipStream_t stream) {
-    auto* blocks = static_cast<int8_t*>(call.workspace);
-    auto* scales = reinterpret_cast<float*>(blocks + int8_block_bytes(call.rows, w.input));
-    const hipError_t e = launch_int8_stage(call.x, call.rows, w.input, call.x_scales, blocks, scales, stream);
-    if (e != hipSuccess) return e;
-    Int8Args a{};
-    a.w = w.blocks;
-    a.x = blocks;
-    a.t = w.scales;
-    a.s = scales;
-    a.bias = w.bias;
-    a.y = const_cast<void*>(call.y.data);
-    a.y_stride = call.y.stride;
-    a.y_type = call.y.type;
-    a.rows = uint32_t(call.rows);
-    a.output = w.output;
-    a.k_blocks = int8_k_blocks(w.input);
-    a.alpha = call.alpha;
-    a.beta = call.beta;
-    if (call.rows <= 16) {
-        hipLaunchKernelGGL(int8_rows16_kernel, dim3((w.output + 15) / 16), dim3(512), 0, stream, a);
-    } else {
-        const uint32_t nt = (w.output + 127) / 128;
-        const uint32_t tiles = nt * uint32_t((call.rows + 127) / 128);
-        hipLaunchKernelGGL(int8_tile_kernel, dim3(tiles), dim3(256), 0, stream, a, nt);
-    }
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 hipError_t launch_int8_linear(const Int8Layer& w, const Int8Call& call, hipStream_t stream) {

@@ -50,9 +50,21 @@ struct Int8Call {
 hipError_t launch_int8_stage(const OpRows& x, uint64_t rows, uint32_t input, const float* given, int8_t* blocks,
                              float* scales, hipStream_t stream);
 hipError_t launch_copy_f32(const float* from, float* to, uint64_t count, hipStream_t stream);
-// Rows of one pass (a launch holds fewer than 2^32 threads: 2^22 tiles of 128 x
-// 128), and the workspace: a pass's activations in blocks, then their scales.
+// Rows of one pass (a launch holds fewer than 2^32 threads).
 uint64_t int8_pass_rows(uint64_t rows, uint32_t output);
+// How a pass of `rows` runs: its core, the core's tiles, and where the scales
+// start in its workspace (the activations' blocks are at 0).
+enum Int8Core : uint32_t {
+    kInt8Decode, kInt8Rows16, kInt8Direct32x32, kInt8Direct32x64, kInt8Direct64x64,   // channels x rows
+    kInt8Wide128x128, kInt8Wide256x128
+};
+struct Int8Plan {
+    Int8Core core = kInt8Decode;
+    uint32_t n_tiles = 0, m_tiles = 0;
+    uint64_t scales_at = 0, bytes = 0;
+};
+constexpr uint32_t kInt8DecodeLds = 44 * 1024;   // rows of a decode launch in LDS, beside 8 KiB of sums
+Int8Plan int8_plan(uint64_t rows, uint32_t input, uint32_t output);
 uint64_t int8_workspace_bytes(uint64_t rows, uint32_t input, uint32_t output);
 hipError_t launch_int8_linear(const Int8Layer& w, const Int8Call& call, hipStream_t stream);
 

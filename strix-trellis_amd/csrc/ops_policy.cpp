@@ -6,14 +6,54 @@
 namespace stx {
 
 uint64_t int8_pass_rows(uint64_t rows, uint32_t output) {
-    const uint64_t n_tiles = (uint64_t(output) + 127) / 128, most = (uint64_t(1) << 22) / n_tiles;
-    const uint64_t pass = 128 * (most < 2048 ? most : 2048);
+    // 64 x 64 tiles of 512 threads: 2^22 of them, 2^16 rows at most
+    const uint64_t n_tiles = (uint64_t(output) + 63) / 64, most = (uint64_t(1) << 22) / n_tiles;
+    const uint64_t pass = 64 * (most < 1024 ? most : 1024);
     return rows < pass ? rows : pass;
 }
 
+Int8Plan int8_plan(uint64_t rows, uint32_t input, uint32_t output) {
+    Int8Plan p;
+    const uint64_t kbs = int8_k_blocks(input), groups = (uint64_t(output) + 15) / 16;
+    // A few rows: every 16-channel workgroup rounds the rows itself, which saves a
+    // launch but costs each of them the rows' reads.  Against the two launches:
+    // 5120^2 one / two rows 6.6 / 7.6 us for 9.5, 4096 -> 12288 four rows 11.2
+    // for 12.8, 1152 -> 5120 eight rows 5.5 for 7.2; but 5120^2 eight rows 12.1
+    // for 8.0, 5120 -> 129280 four rows 137 for 117 (one row 103 for 114).
+    const bool decode = rows == 1 || (rows <= 4 && rows * groups <= 4096) || (rows <= 8 && input <= 1536);
+    if (decode && rows * (kbs * 64 + 64) <= kInt8DecodeLds) return p;   // needs no workspace
+    p.scales_at = int8_block_bytes(rows, input);
+    p.bytes = (p.scales_at + rows * 4 + 255) & ~uint64_t(255);
+    auto tile = [&](Int8Core core, uint32_t channels, uint32_t tile_rows) {
+        p.core = core;
+        p.n_tiles = (output + channels - 1) / channels;
+        p.m_tiles = uint32_t((rows + tile_rows - 1) / tile_rows);
+        return uint64_t(p.n_tiles) * p.m_tiles;
+    };
+    if (rows <= 16) {
+        tile(kInt8Rows16, 16, 16);
+        return p;
+    }
+    // The smallest direct tile whose workgroups (one per compute unit at a time)
+    // fill one round: 5120^2 48 rows 12.1 us in 32 x 64 tiles, 16.3 in 32 x 32 (two
+    // rounds), 15.0 in 64 x 64; 4096 -> 12288 48 rows 16.8 in 64 x 64, 20.1 in 32
+    // x 64, 21.3 in 32 x 32.  Up to 32 rows one and a half rounds of the smallest
+    // are faster than one of the next (4096 -> 12288 14.2 us for 16.1).
+    if (rows <= 64) {
+        if (tile(kInt8Direct32x32, 32, 32) <= (rows <= 32 ? 384 : 256)) return p;
+        if (tile(kInt8Direct32x64, 32, 64) <= 256) return p;
+    }
+    // Past one round, LDS tiles: 5120^2 192 / 512 rows 16.7 / 39.5 us direct, 26.0 /
+    // 29.9 in 128 x 128 tiles; 4096 -> 12288 256 rows 39.8 and 24.8.
+    if (tile(kInt8Direct64x64, 64, 64) <= 256) return p;
+    // The larger LDS tile where it still fills two rounds: 4096 -> 12288 2048 rows
+    // 112 us in 128 x 128, 107 in 256 x 128; 1024 rows 61 and 66.
+    if (tile(kInt8Wide256x128, 256, 128) < 640) tile(kInt8Wide128x128, 128, 128);
+    return p;
+}
+
 uint64_t int8_workspace_bytes(uint64_t rows, uint32_t input, uint32_t output) {
-    rows = int8_pass_rows(rows, output);
-    return int8_block_bytes(rows, input) + (rows * 4 + 255) / 256 * 256;
+    return int8_plan(int8_pass_rows(rows, output), input, output).bytes;
 }
 
 // Enough workgroups for few rows, whole batches each.

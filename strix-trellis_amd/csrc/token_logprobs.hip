@@ -2,23 +2,29 @@
 // probability and rank of a given token, the entropy, and the most likely
 // tokens, in one pass over the logits.
 //
-// Running statistics.  With m the largest logit so far, c = scale, a thread
-// holds n = the count of logits equal to m, and over the others
+// Running statistics.  With m the largest logit so far, c = scale, a wave holds
+// n = the count of logits equal to m, and over the others
 //   s = sum e^(c (x - m))      h = sum e^(c (x - m)) c (x - m)
 // so that log sum = log n + log1p(s / n) and entropy = log sum - h / (n + s)
 // keep their relative precision where one token takes nearly everything.  h is
 // held in units of log2 e.  Logits of -inf add nothing: m starts at the
-// lowest finite float.
+// lowest finite float.  m is the wave's, so a batch whose largest logit stays
+// below it (nearly all of them) needs neither a rescaling nor a count.
+//
+// Rank.  Tokens ahead of the given one are those of at least its logit before
+// it and of more than its logit behind it: one comparison per logit, with a
+// bound that changes once.
 //
 // Most likely tokens.  A token's place in the order is one 64-bit key: the
 // logit's bits, made monotonic, over the inverted id, so larger keys come
 // first and equal logits go by the lower id.  The workgroup keeps a list of
 // candidates in LDS and a bound that at least `top` keys reach; a token
 // enters the list if it reaches the bound.  The first batch takes its bound
-// from the threads' largest tokens (the k-th largest of each wave, with k * waves
-// >= top), and whenever the list has grown it is cut to the first `top` keys,
-// the last of which is the new bound.  Only a few dozen of 10^5 tokens ever
-// enter.
+// from the threads' largest logits (the k-th largest of each wave, with k * waves
+// >= top).  Behind batches 1, 2, 4, 8, .. the list is cut to the first `top`
+// keys, the last of which is the new bound: about `top` tokens enter between two
+// cuts, and the waves meet only there.  A list that overflowed in between
+// (rising or equal logits) is filled again from memory, with a higher bound.
 #include "ops_device.hpp"
 
 namespace stx {
@@ -29,10 +35,9 @@ constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kEach = 16;                               // logits per thread and batch
 constexpr uint32_t kBatch = kThreads * kEach;
 static_assert(kBatch == kLogprobsBatch);
-constexpr uint32_t kList = 1024;                        // candidate capacity, above the most `top`
-constexpr uint32_t kCut = 256;                          // list length that is cut at the end of a batch
+constexpr uint32_t kList = 1024;                        // candidate capacity
 constexpr float kLn2 = 0.69314718055994530942f;
-constexpr float kLowest = -3.40282346638528859812e38f;
+constexpr float kLowest = -3.40282346638528859812e38f, kInf = __builtin_inff();
 
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t id) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);   // -0 counts as 0
@@ -44,37 +49,36 @@ __device__ __forceinline__ float value_of(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t id_of(uint64_t key) { return ~uint32_t(key); }
 
+// The next float above x (x not NaN or +inf).
+__device__ __forceinline__ float above(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
+    return __builtin_bit_cast(float, b & 0x80000000u ? b - 1 : b + 1);
+}
+
 struct Stats {
     float m, n, s, h;
 };
 constexpr Stats kNothing = {kLowest, 0.0f, 0.0f, 0.0f};
 
-// c as a sum of two floats times log2 e: exponents of 2 without a rounding that
-// grows with the distance.
-struct Scale {
-    float hi, lo;
-};
 // Distances past 2^24 have no weight at any admitted scale (2^24 times 2^-16
-// log2 e is over 300); kept finite, a weight of 0 times one is 0.  NaN stays NaN.
-__device__ __forceinline__ float power(float d, Scale c) {
-    d = __builtin_elementwise_maximum(d, -0x1p24f);
-    return __builtin_fmaf(d, c.hi, d * c.lo);
-}
+// log2 e is over 300); kept finite, a weight of 0 times one is 0.
+__device__ __forceinline__ float power(float d, float c) { return fmaxf(d, -0x1p24f) * c; }
 
-// Joins b into a.
-__device__ __forceinline__ void join(Stats& a, const Stats& b, Scale c) {
+// Statistics p against the larger maximum m.
+__device__ __forceinline__ Stats against(const Stats& p, float m, float c) {
+    const float d = power(p.m - m, c), f = __builtin_amdgcn_exp2f(d), t = p.n + p.s;
+    return p.m == m ? p : Stats{m, 0.0f, f * t, f * __builtin_fmaf(t, d, p.h)};
+}
+__device__ __forceinline__ void join(Stats& a, const Stats& b, float c) {
     const float m = fmaxf(a.m, b.m);
-    auto part = [&](const Stats& p) {
-        Stats q = p;
-        if (p.m == m) return q;
-        const float d = power(p.m - m, c), f = exp2f(d), t = p.n + p.s;
-        q.n = 0.0f;
-        q.s = f * t;
-        q.h = f * __builtin_fmaf(t, d, p.h);
-        return q;
-    };
-    const Stats x = part(a), y = part(b);
+    const Stats x = against(a, m, c), y = against(b, m, c);
     a = {m, x.n + y.n, x.s + y.s, x.h + y.h};
+}
+// Joins the lanes' statistics; every lane gets the result.
+__device__ __forceinline__ Stats join_lanes(const Stats& mine, float c) {
+    const float m = wave_max(mine.m);
+    const Stats x = against(mine, m, c);
+    return {m, wave_sum(x.n), wave_sum(x.s), wave_sum(x.h)};
 }
 
 // What the statistics of a whole row say; invalid rows give NaN.
@@ -84,7 +88,7 @@ struct Answer {
 };
 __device__ __forceinline__ Answer answer_of(const Stats& t) {
     Answer a;
-    a.valid = t.n > 0.0f && t.m < __builtin_inff() && t.s == t.s;
+    a.valid = t.n > 0.0f && t.m < kInf && t.s == t.s;
     a.log_sum = logf(t.n) + log1pf(t.s / t.n);
     a.entropy = a.log_sum - t.h * kLn2 / (t.n + t.s);
     return a;
@@ -100,8 +104,7 @@ struct Args {
     int32_t* top_ids;
     float* top_logprobs;
     uint32_t vocab, top, splits, split_length;
-    float scale;
-    Scale c;
+    float scale, c;           // c = scale log2 e
     // splits > 1: per row and split the statistics and the tokens ahead
     // ([rows][splits][8] words), then the keys ([rows][splits][top]).
     float* part;
@@ -110,27 +113,31 @@ struct Args {
 
 // Sorts the first `top` of list[0..count) to its front (largest first) and
 // returns how many there are.  All threads call it; ends with a barrier.
-// Ranks by counting: every key is distinct.
+// Ranks by counting (every key is distinct), eight keys of the list in flight
+// per step; keys past the count are 0, which is ahead of none.
 __device__ __forceinline__ uint32_t cut(uint64_t* list, uint32_t count, uint32_t top) {
-    constexpr int kMine = kList / kThreads;
-    uint64_t mine[kMine];
-    uint32_t ahead[kMine] = {};
+    typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+    const uint32_t i0 = threadIdx.x, i1 = threadIdx.x + kThreads, padded = (count + 7) & ~7u;
+    if (count + i0 < padded) list[count + i0] = 0;
+    __syncthreads();
+    const uint64_t k0 = i0 < count ? list[i0] : 0, k1 = i1 < count ? list[i1] : 0;
+    uint32_t a0 = 0, a1 = 0;
+    if (uint32_t(__builtin_amdgcn_readfirstlane(i0)) < count) {   // the wave holds keys
+        for (uint32_t i = 0; i < padded; i += 8) {
+            u64x2 k[4];
 #pragma unroll
-    for (int j = 0; j < kMine; ++j) {
-        const uint32_t i = threadIdx.x + j * kThreads;
-        mine[j] = i < count ? list[i] : 0;
-    }
-    if (threadIdx.x < count) {
-        for (uint32_t i = 0; i < count; ++i) {
-            const uint64_t k = list[i];
+            for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const u64x2*>(list + i + 2 * j);
 #pragma unroll
-            for (int j = 0; j < kMine; ++j) ahead[j] += k > mine[j];
+            for (int j = 0; j < 4; ++j) a0 += (k[j][0] > k0) + (k[j][1] > k0);
+            if (count > kThreads) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) a1 += (k[j][0] > k1) + (k[j][1] > k1);
+            }
         }
     }
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kMine; ++j)
-        if (threadIdx.x + j * kThreads < count && ahead[j] < top) list[ahead[j]] = mine[j];
+    if (i0 < count && a0 < top) list[a0] = k0;
+    if (i1 < count && a1 < top) list[a1] = k1;
     __syncthreads();
     return count < top ? count : top;
 }
@@ -162,148 +169,220 @@ __device__ __forceinline__ void finish(const Args& a, uint64_t row, const Stats&
     }
 }
 
+// A thread's logits of a batch as loaded: groups of 16 bytes, the workgroup's
+// groups side by side.
 template <class T>
-__global__ __launch_bounds__(kThreads) void token_logprobs_kernel(Args a) {
-    __shared__ uint64_t list[kList];
-    __shared__ uint64_t wave_key[kWaves];
+struct Batch {
+    static constexpr int kGroup = 16 / sizeof(T), kGroups = kEach / kGroup;
+    typename Packed<T, kGroup>::type raw[kGroups];
+
+    static __device__ __forceinline__ uint32_t first(int g) { return (g * kThreads + threadIdx.x) * kGroup; }
+    // A group that would reach past v1 is loaded where it ends at v1: its first
+    // logits are another group's, and drop out by `id`.
+    static __device__ __forceinline__ uint32_t place(uint32_t b0, uint32_t v1, int g) {
+        const uint32_t k = b0 + first(g);
+        return k < v1 - kGroup ? k : v1 - kGroup;
+    }
+    __device__ __forceinline__ void load(const T* x, uint32_t b0, uint32_t v1) {
+        if (b0 + kBatch <= v1) {
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) raw[g] = ld_packed<kGroup>(x + b0 + first(g));
+        } else if (v1 >= uint32_t(kGroup)) {
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) raw[g] = ld_packed<kGroup>(x + place(b0, v1, g));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kGroup; ++i) raw[0][i] = uint32_t(i) < v1 ? ld_global(x + i) : T(-kInf);
+        }
+    }
+    // Token of element e, ~0 where another element is that token or there is none.
+    static __device__ __forceinline__ uint32_t id(uint32_t b0, uint32_t v1, int e) {
+        const uint32_t k = b0 + first(e / kGroup);
+        if (b0 + kBatch <= v1) return k + e % kGroup;
+        if (v1 < uint32_t(kGroup)) return k + e % kGroup < v1 ? k + e % kGroup : ~0u;
+        const uint32_t i = place(b0, v1, e / kGroup) + e % kGroup;
+        return i >= k ? i : ~0u;
+    }
+    // The logits, -inf where `id` gives none.
+    __device__ __forceinline__ void values(uint32_t b0, uint32_t v1, float (&v)[kEach]) const {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) v[e] = float(raw[e / kGroup][e % kGroup]);
+        if (b0 + kBatch > v1) {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) v[e] = id(b0, v1, e) != ~0u ? v[e] : -kInf;
+        }
+    }
+};
+
+template <class T>
+__global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(Args a) {
+    __shared__ __align__(16) uint64_t list[kList];
+    __shared__ float wave_bound[kWaves];
     __shared__ Stats wave_stats[kWaves];
     __shared__ uint32_t wave_ahead[kWaves];
-    __shared__ uint32_t list_count;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    __shared__ uint32_t list_end;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint64_t row = blockIdx.x / a.splits;
     const uint32_t split = blockIdx.x % a.splits, v0 = split * a.split_length;
     const uint32_t v1 = a.vocab - v0 < a.split_length ? a.vocab : v0 + a.split_length;
     const T* x = static_cast<const T*>(a.logits) + row * a.stride;
-    int32_t token = a.tokens ? ld_global(a.tokens + row) : -1;
-    const bool have_token = uint32_t(token) < a.vocab;
-    const float given = have_token ? float(ld_global(x + token)) : __builtin_inff();
-    Stats t = kNothing;
-    uint32_t ahead = 0;
+    using B = Batch<T>;
+    B batch, next, later;   // two batches ahead: a round trip to memory takes longer than a batch
+    batch.load(x, v0, v1);
+    if (v0 + kBatch < v1) next.load(x, v0 + kBatch, v1);
+    const uint32_t token = a.tokens ? uint32_t(ld_global(a.tokens + row)) : ~0u;
+    const float given = token < a.vocab ? float(ld_global(x + token)) : kInf;
+    Stats t = kNothing;        // m is the wave's
+    uint32_t ahead = 0;        // the wave's
+    bool bad = false;          // a NaN
     uint64_t bound = 0;        // keys below it do not enter the list
-    uint32_t count = 0;        // length of the list, the same in every thread
-    if (tid == 0) list_count = 0;
+    float reach = -kInf;       // its logit
+    uint32_t count = 0;        // keys in the list behind the last cut
+    float peak = -kInf;        // the thread's largest logit since then
+    uint32_t since = v0, cut_at = v0;   // the first batch since then, the batch behind which the next cut comes
+    if (tid == 0) list_end = 0;
 
-    for (uint32_t b0 = v0; b0 < v1; b0 += kBatch) {
-        // logits 4 j .. 4 j + 3 of the thread's four groups, 4 kThreads apart
-        float v[kEach];
-#pragma unroll
-        for (int j = 0; j < kEach / 4; ++j) {
-            float q[4];
-            load_row<4>(x, b0 + (j * kThreads + tid) * 4, v1, -__builtin_inff(), q);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * j + i] = q[i];
-        }
-        auto id_at = [&](int e) { return b0 + ((e >> 2) * kThreads + tid) * 4 + (e & 3); };
-
-        // ---- statistics ----
-        float most = t.m;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) most = fmaxf(most, v[e]);
-        if (most > t.m) {
-            const float d = power(t.m - most, a.c), f = exp2f(d), all = t.n + t.s;
-            t = {most, 0.0f, f * all, f * __builtin_fmaf(all, d, t.h)};
-        }
+    auto enter = [&](uint32_t b0, const float (&v)[kEach]) {
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const float d = power(v[e] - t.m, a.c);
-            const float p = v[e] == t.m ? 0.0f : exp2f(d);
-            t.n += v[e] == t.m ? 1.0f : 0.0f;
-            t.s += p;
-            t.h = __builtin_fmaf(p, d, t.h);
+            if (!__any(v[e] >= reach)) continue;
+            const uint32_t id = B::id(b0, v1, e);
+            const uint64_t k = key_of(v[e], id);
+            if (v[e] >= reach && k >= bound && id != ~0u) {
+                const uint32_t slot = atomicAdd(&list_end, 1u);
+                if (slot < kList) list[slot] = k;
+            }
         }
-        if (have_token) {
+    };
+    // A logit that at least `top` of the tokens since `since` reach, or -inf: the
+    // k-th largest peak of each wave of which every lane has tokens, the least
+    // of them.  Ends with a barrier.
+    auto reach_of_peaks = [&] {
+        const uint32_t tokens = v1 - since, of_wave = tokens / (64 * B::kGroup);
+        const uint32_t waves = of_wave < 1 ? 1 : of_wave < kWaves ? of_wave : kWaves;
+        float left = peak, kth = -kInf;
+        for (uint32_t k = (a.top + waves - 1) / waves; k; --k) {
+            kth = wave_max(left);
+            const uint64_t at = __ballot(left == kth);
+            if (at && lane == __builtin_ctzll(at)) left = -kInf;
+        }
+        if (lane == 0) wave_bound[w] = uint32_t(w) < waves ? kth : kInf;
+        __syncthreads();
+        float least = wave_bound[0];
 #pragma unroll
-            for (int e = 0; e < kEach; ++e)
-                ahead += v[e] > given || (v[e] == given && id_at(e) < uint32_t(token));
-        }
-        if (!a.top) continue;
+        for (int i = 1; i < kWaves; ++i) least = fminf(least, wave_bound[i]);
+        __syncthreads();
+        return least;
+    };
 
-        // ---- candidates ----
-        if (b0 == v0) {
-            // The bound of the first batch: every wave's k-th largest thread
-            // key, the least of them.  A thread without a token has key 0.
-            uint64_t best = 0;
+    for (uint32_t b0 = v0; b0 < v1; b0 += kBatch) {
+        if (v1 - b0 > 2 * kBatch) later.load(x, b0 + 2 * kBatch, v1);
+        float v[kEach];
+        batch.values(b0, v1, v);
+
+        // ---- statistics ----
+        float most = v[0];   // NaN if one is among them
+#pragma unroll
+        for (int e = 1; e < kEach; ++e) most = __builtin_elementwise_maximum(most, v[e]);
+        bad |= most != most;
+        const float wave_most = wave_max(most);
+        if (wave_most >= t.m) {   // the wave as one
+            t = against(t, wave_most, a.c);
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
-                const uint64_t k = id_at(e) < v1 ? key_of(v[e], id_at(e)) : 0;
-                best = k > best ? k : best;
+                const float d = power(v[e] - t.m, a.c), p = v[e] == t.m ? 0.0f : __builtin_amdgcn_exp2f(d);
+                t.n += v[e] == t.m ? 1.0f : 0.0f;
+                t.s += p;
+                t.h = __builtin_fmaf(p, d, t.h);
             }
-            const uint32_t kth = (a.top + kWaves - 1) / kWaves - 1;
-            uint32_t before = 0;   // keys of the wave ahead of this one (equal zero keys: by lane)
-            for (int l = 0; l < 64; ++l) {
-                const uint64_t o = __shfl(best, l);
-                before += o > best || (o == best && l < lane);
-            }
-            if (before == kth) wave_key[w] = best;
-            __syncthreads();
-            uint64_t least = wave_key[0];
+        } else {
 #pragma unroll
-            for (int i = 1; i < kWaves; ++i) least = wave_key[i] < least ? wave_key[i] : least;
-            bound = least;
+            for (int e = 0; e < kEach; ++e) {
+                const float d = power(v[e] - t.m, a.c), p = __builtin_amdgcn_exp2f(d);
+                t.s += p;
+                t.h = __builtin_fmaf(p, d, t.h);
+            }
         }
-        for (;;) {
-            const float reach = bound ? value_of(bound) : -__builtin_inff();
-            uint32_t enter = 0;
+        // ---- rank ----
+        if (token < a.vocab) {
+            if (token - b0 < kBatch) {
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) enter |= uint32_t(v[e] >= reach) << e;
-            if (enter) {
+                for (int e = 0; e < kEach; ++e)
+                    ahead += __popcll(__ballot(v[e] > given || (v[e] == given && B::id(b0, v1, e) < token)));
+            } else {
+                const float least = b0 < token ? given : above(given);
 #pragma unroll
-                for (int e = 0; e < kEach; ++e) {
-                    if (!(enter >> e & 1) || id_at(e) >= v1) continue;
-                    const uint64_t k = key_of(v[e], id_at(e));
-                    if (k < bound) continue;
-                    const uint32_t slot = atomicAdd(&list_count, 1u);
-                    if (slot < kList) list[slot] = k;
+                for (int e = 0; e < kEach; ++e) ahead += __popcll(__ballot(v[e] >= least));
+            }
+        }
+        // ---- candidates ----
+        if (a.top) {
+            peak = fmaxf(peak, most);
+            if (b0 == v0) {
+                reach = reach_of_peaks();
+                bound = uint64_t(key_of(reach, 0) >> 32) << 32;   // every id of that logit
+            }
+            if (__any(most >= reach)) enter(b0, v);
+            const bool last = v1 - b0 <= kBatch;
+            if (b0 == cut_at || last) {
+                __syncthreads();
+                while (list_end > kList) {
+                    // More tokens than the list holds.  The peaks or, with many
+                    // equal logits, the keys that got in give a higher bound; the
+                    // batches since the last cut enter again behind its keys.  By
+                    // the list's own bound at least kList - 2 top keys fewer do
+                    // each time.
+                    const uint64_t kept = uint32_t(tid) < count ? list[tid] : 0;
+                    const float higher = reach_of_peaks();
+                    cut(list, kList, a.top);
+                    const uint64_t of_list = list[a.top - 1], of_peaks = uint64_t(key_of(higher, 0) >> 32) << 32;
+                    bound = of_list > of_peaks ? of_list : of_peaks;
+                    reach = value_of(bound);
+                    __syncthreads();
+                    if (uint32_t(tid) < count) list[tid] = kept;
+                    if (tid == 0) list_end = count;
+                    __syncthreads();
+                    for (uint32_t b = since; b <= b0; b += kBatch) {
+                        B again;
+                        again.load(x, b, v1);
+                        float u[kEach];
+                        again.values(b, v1, u);
+                        enter(b, u);
+                    }
+                    __syncthreads();
+                }
+                count = cut(list, list_end, a.top);
+                if (!last) {
+                    if (count == a.top) {
+                        bound = list[a.top - 1];
+                        reach = value_of(bound);
+                    }
+                    if (tid == 0) list_end = count;
+                    since = b0 + kBatch;
+                    cut_at += cut_at - v0 + kBatch;   // behind batch 0, 1, 3, 7, ..
+                    peak = -kInf;
+                    __syncthreads();
                 }
             }
-            __syncthreads();
-            const uint32_t entered = list_count;
-            __syncthreads();
-            if (entered <= kList) {
-                count = entered;
-                break;
-            }
-            // More tokens than the list holds (many equal ones): the keys that
-            // got in give a higher bound; the list goes back to the earlier
-            // batches' keys, which all stay within the first `top` slots, and
-            // the batch enters again.  Each time at least kList - top fewer do.
-            uint64_t kept = tid < int(count) ? list[tid] : 0;   // count <= kCut < kThreads here
-            __syncthreads();
-            cut(list, kList, a.top);
-            bound = list[a.top - 1];
-            __syncthreads();
-            if (tid < int(count)) list[tid] = kept;
-            if (tid == 0) list_count = count;
-            __syncthreads();
         }
-        if (count > kCut && b0 + kBatch < v1) {
-            count = cut(list, count, a.top);
-            if (count == a.top) bound = list[a.top - 1];
-            if (tid == 0) list_count = count;
-            __syncthreads();
-        }
+        batch = next;
+        next = later;
     }
 
     // ---- the row's or the split's results ----
-    // a +inf or NaN row: m is +inf or s NaN, whichever thread saw it
-#pragma unroll
-    for (int s = 32; s; s >>= 1) {
-        const Stats o = {__shfl_xor(t.m, s), __shfl_xor(t.n, s), __shfl_xor(t.s, s), __shfl_xor(t.h, s)};
-        join(t, o, a.c);
-        ahead += __shfl_xor(ahead, s);
-    }
+    if (bad) t.s = __builtin_nanf("");
+    t.n = wave_sum(t.n);
+    t.s = wave_sum(t.s);
+    t.h = wave_sum(t.h);
     if (lane == 0) {
         wave_stats[w] = t;
         wave_ahead[w] = ahead;
     }
     __syncthreads();
-    t = wave_stats[0];
-    ahead = wave_ahead[0];
-    for (int i = 1; i < kWaves; ++i) {
-        join(t, wave_stats[i], a.c);
-        ahead += wave_ahead[i];
-    }
-    if (a.top) count = cut(list, count, a.top);
+    t = join_lanes(lane < kWaves ? wave_stats[lane & (kWaves - 1)] : kNothing, a.c);
+    ahead = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) ahead += wave_ahead[i];
     if (a.splits == 1) {
         finish<T>(a, row, t, ahead, list);
         return;
@@ -311,10 +390,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(Args a) {
     const uint64_t p = row * a.splits + split;
     if (tid == 0) {
         float* to = a.part + p * 8;
-        st_global(to, t.m);
-        st_global(to + 1, t.n);
-        st_global(to + 2, t.s);
-        st_global(to + 3, t.h);
+        st_global(reinterpret_cast<f32x4*>(to), f32x4{t.m, t.n, t.s, t.h});
         st_global(reinterpret_cast<uint32_t*>(to + 4), ahead);
     }
     // only the last split can be shorter than `top`: its keys end the row's
@@ -324,30 +400,38 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(Args a) {
 // Joins the splits of a row.
 template <class T>
 __global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(Args a) {
-    __shared__ uint64_t list[kList];
+    __shared__ __align__(16) uint64_t list[kList];
     const uint64_t row = blockIdx.x, p = row * a.splits;
+    const uint32_t tid = threadIdx.x, last = a.vocab - (a.splits - 1) * a.split_length;
+    const uint32_t keys = a.top ? (a.splits - 1) * a.top + (last < a.top ? last : a.top) : 0;
+    const uint64_t* from = a.part_keys + p * a.top;
+    // the list in rounds, as many keys at a time as it holds
+    uint32_t count = keys < kList ? keys : kList, taken = count;
+    for (uint32_t i = tid; i < count; i += kThreads) list[i] = ld_global(from + i);
     Stats t = kNothing;
-    uint32_t ahead = 0;
-    for (uint32_t i = 0; i < a.splits; ++i) {
-        const float* from = a.part + (p + i) * 8;
-        const Stats o = {ld_global(from), ld_global(from + 1), ld_global(from + 2), ld_global(from + 3)};
-        join(t, o, a.c);
-        ahead += ld_global(reinterpret_cast<const uint32_t*>(from + 4));
+    float ahead = 0;   // whole numbers of a row's tokens: two halves, each exact in a float sum
+    float ahead_high = 0;
+    for (uint32_t i = tid & 63; i < a.splits; i += 64) {
+        const f32x4 o = ld_global(reinterpret_cast<const f32x4*>(a.part + (p + i) * 8));
+        const uint32_t n = ld_global(reinterpret_cast<const uint32_t*>(a.part + (p + i) * 8 + 4));
+        join(t, {o[0], o[1], o[2], o[3]}, a.c);
+        ahead += float(n & 0x3FFFu);
+        ahead_high += float(n >> 14);
     }
+    t = join_lanes(t, a.c);
+    const uint32_t total = uint32_t(wave_sum(ahead)) + (uint32_t(wave_sum(ahead_high)) << 14);
+    __syncthreads();
     if (a.top) {
-        // the list in rounds, as many splits at a time as it holds
-        uint32_t count = 0;
-        const uint32_t last = a.vocab - (a.splits - 1) * a.split_length;
-        const uint32_t keys = (a.splits - 1) * a.top + (last < a.top ? last : a.top);
-        for (uint32_t i = 0; i < keys;) {
-            const uint32_t n = keys - i < kList - count ? keys - i : kList - count;
-            for (uint32_t j = threadIdx.x; j < n; j += kThreads) list[count + j] = ld_global(a.part_keys + p * a.top + i + j);
+        count = cut(list, count, a.top);
+        while (taken < keys) {
+            const uint32_t n = keys - taken < kList - count ? keys - taken : kList - count;
+            for (uint32_t i = tid; i < n; i += kThreads) list[count + i] = ld_global(from + taken + i);
             __syncthreads();
             count = cut(list, count + n, a.top);
-            i += n;
+            taken += n;
         }
     }
-    finish<T>(a, row, t, ahead, list);
+    finish<T>(a, row, t, total, list);
 }
 
 template <class T>
@@ -374,9 +458,7 @@ hipError_t launch_token_logprobs(const LogprobsCall& call, hipStream_t stream) {
     a.vocab = call.vocab;
     a.top = call.top;
     a.scale = call.scale;
-    const double c = double(call.scale) * 1.4426950408889634074;
-    a.c.hi = float(c);
-    a.c.lo = float(c - double(a.c.hi));
+    a.c = float(double(call.scale) * 1.4426950408889634074);
     const uint64_t batches = (uint64_t(call.vocab) + kBatch - 1) / kBatch;
     a.splits = logprobs_splits(call.rows, call.vocab);
     a.split_length = uint32_t((batches + a.splits - 1) / a.splits) * kBatch;

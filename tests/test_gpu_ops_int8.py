@@ -254,7 +254,8 @@ def test_refusals(ctx):
     assert status(x.to(torch.int8), y) == "INSUFFICIENT_BUFFER"
     assert status(x.to(torch.int8), y, x_scales=torch.ones(3, device=DEV)) == "INSUFFICIENT_BUFFER"
     assert status(x, y, alpha=float("inf")) == "INVALID_ARGUMENT"
-    assert status(x, y, workspace=torch.zeros(256, dtype=torch.uint8, device=DEV)) == "INSUFFICIENT_BUFFER"
+    many = torch.randn(20, 64, device=DEV), torch.zeros(20, 32, device=DEV)
+    assert status(*many, workspace=torch.zeros(256, dtype=torch.uint8, device=DEV)) == "INSUFFICIENT_BUFFER"
     assert status(x.cpu(), y, workspace=torch.zeros(1 << 16, dtype=torch.uint8, device=DEV)) == "INVALID_ARGUMENT"
     both = torch.zeros(4, 96, device=DEV)
     assert status(both[:, :64], both[:, 32:64]) == "INVALID_ARGUMENT"
