@@ -28,13 +28,20 @@ __device__ __forceinline__ float group_sum(float v, float* slot) {
 
 // A thread's share of a row (or of a vector): groups of four channels, the
 // workgroup's groups side by side.  Every group but the last lies inside the
-// row: C is the least that covers the width.
+// row: C is the least that covers the width.  A wave whose last group lies
+// behind the row leaves it out (`tail`, uniform).
+template <int THREADS, int C>
+__device__ __forceinline__ bool tail_of_wave(uint32_t width) {
+    return ((C - 1) * THREADS + __builtin_amdgcn_readfirstlane(threadIdx.x & ~63u)) * 4 < width;
+}
 template <class T, int THREADS, int C>
 struct Share {
     Raw4<T> raw[C];
     __device__ __forceinline__ void load(const T* row, uint32_t width) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) raw[c] = load4(row, (c * THREADS + threadIdx.x) * 4, width, c + 1 < C);
+        for (int c = 0; c + 1 < C; ++c) raw[c] = load4(row, (c * THREADS + threadIdx.x) * 4, width, true);
+        if (tail_of_wave<THREADS, C>(width)) raw[C - 1] = load4(row, ((C - 1) * THREADS + threadIdx.x) * 4, width, false);
+        else raw[C - 1].v = typename Packed<T, 4>::type{};
     }
 };
 
@@ -97,6 +104,7 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormCall a) {
     Share<T, THREADS, C> block, residual, gate;
     Share<float, THREADS, C> post, pre, post_bias, pre_bias, channel;
     constexpr bool EARLY = LOADS != kLate, ALL = LOADS == kAll;
+    const bool tail = tail_of_wave<THREADS, C>(width);
     const bool full_gate = a.gate.data && !a.gate_per_row;
     float row_gate = 1.0f;
     if (a.block.data) block.load(at(a.block), width);
@@ -116,10 +124,11 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormCall a) {
         if (a.post_weight)
             normalise<THREADS>(v, a, post, EARLY ? nullptr : a.post_weight, post_bias, a.post_bias, !ALL, slots);
         if (!EARLY && full_gate) gate.load(at(a.gate), width);
-        auto act = [&](float g) { return a.sigmoid ? 1.0f / (1.0f + expf(-g)) : g; };
+        auto act = [&](float g) { return a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + expf(-g)) : g; };
         if (!full_gate) row_gate = a.block_scale * (a.gate.data ? act(row_gate) : 1.0f);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
+            if (c + 1 == C && !tail) continue;
             float g[4];
             if (full_gate) gate.raw[c].to(g);
 #pragma unroll
@@ -150,7 +159,8 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormCall a) {
     auto store = [&](const OpRows& to) {
         T* out = const_cast<T*>(at(to));
 #pragma unroll
-        for (int c = 0; c < C; ++c) store4(out, (c * THREADS + threadIdx.x) * 4, width, v[c]);
+        for (int c = 0; c < C; ++c)
+            if (c + 1 < C || tail) store4(out, (c * THREADS + threadIdx.x) * 4, width, v[c]);
     };
     if (a.hidden.data) store(a.hidden);
     if (!a.normed.data) return;

@@ -354,7 +354,10 @@ __global__ __launch_bounds__(512, 2) void int8_direct_kernel(Int8Args a) {
     constexpr int kUnits = BN / 4, kPlane = BM * BN * 4;
     extern __shared__ __align__(16) unsigned char smem[];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const uint32_t nt = blockIdx.x % a.n_tiles, mt = blockIdx.x / a.n_tiles;
+    // The row tiles of a channel tile run on one XCD (workgroup i on XCD i % 8), whose
+    // L2 then reads the weights once.
+    const uint32_t j = blockIdx.x / 8, nt = j / a.m_tiles * 8 + blockIdx.x % 8, mt = j % a.m_tiles;
+    if (nt >= a.n_tiles) return;
     const uint32_t kbs = a.k_blocks, kb0 = kbs * w / 8, kb1 = kbs * (w + 1) / 8, pair = kbs * 1024;
     const uint32_t nb = (a.output + 31) / 32 * 2 - nt * 2 * TN, mb = (a.rows + 31) / 32 * 2 - mt * 2 * TM;
     // blocks of channels or rows past the last read zeros
@@ -606,21 +609,6 @@ hipError_t launch_core(F kernel, uint32_t tiles, uint32_t threads, size_t lds, c
 using Wide256x128 = WideShape<4, 2, 3>;
 using Wide128x128 = WideShape<2, 2, 3>;
 
-// Kernels with more than 64 KiB of LDS have to be told, once.
-hipError_t allow_lds() {
-    static const hipError_t status = [] {
-        const std::pair<void (*)(Int8Args), size_t> large[] = {{int8_direct_kernel<2, 2>, 8 * 16384},
-                                                               {int8_wide_kernel<4, 2, 3>, Wide256x128::kLds}};
-        for (const auto& [kernel, lds] : large) {
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
-            if (e != hipSuccess) return e;
-        }
-        return hipSuccess;
-    }();
-    return status;
-}
-
 hipError_t launch_pass(const Int8Layer& w, const Int8Call& call, hipStream_t stream) {
     const Int8Plan plan = int8_plan(call.rows, w.input, w.output);
     auto* blocks = static_cast<int8_t*>(call.workspace);
@@ -651,15 +639,14 @@ hipError_t launch_pass(const Int8Layer& w, const Int8Call& call, hipStream_t str
     }
     auto* scales = reinterpret_cast<float*>(blocks + plan.scales_at);
     a.s = scales;
-    hipError_t e = allow_lds();
-    if (e == hipSuccess) e = launch_int8_stage(call.x, call.rows, w.input, call.x_scales, blocks, scales, stream);
+    const hipError_t e = launch_int8_stage(call.x, call.rows, w.input, call.x_scales, blocks, scales, stream);
     if (e != hipSuccess) return e;
-    const uint32_t tiles = plan.n_tiles * plan.m_tiles;
+    const uint32_t tiles = plan.n_tiles * plan.m_tiles, spread = (plan.n_tiles + 7) / 8 * 8 * plan.m_tiles;
     switch (plan.core) {
         case kInt8Rows16: return launch_core(int8_rows16_kernel, tiles, 512, 0, a, stream);
-        case kInt8Direct32x32: return launch_core(int8_direct_kernel<1, 1>, tiles, 512, 8 * 4096, a, stream);
-        case kInt8Direct32x64: return launch_core(int8_direct_kernel<1, 2>, tiles, 512, 8 * 8192, a, stream);
-        case kInt8Direct64x64: return launch_core(int8_direct_kernel<2, 2>, tiles, 512, 8 * 16384, a, stream);
+        case kInt8Direct32x32: return launch_core(int8_direct_kernel<1, 1>, spread, 512, 8 * 4096, a, stream);
+        case kInt8Direct32x64: return launch_core(int8_direct_kernel<1, 2>, spread, 512, 8 * 8192, a, stream);
+        case kInt8Direct64x64: return launch_core(int8_direct_kernel<2, 2>, spread, 512, 8 * 16384, a, stream);
         case kInt8Wide256x128: return launch_core(int8_wide_kernel<4, 2, 3>, tiles, 256, Wide256x128::kLds, a, stream);
         case kInt8Wide128x128: return launch_core(int8_wide_kernel<2, 2, 3>, tiles, 256, Wide128x128::kLds, a, stream);
         default: return hipErrorInvalidValue;
@@ -667,6 +654,17 @@ hipError_t launch_pass(const Int8Layer& w, const Int8Call& call, hipStream_t str
 }
 
 }  // namespace
+
+hipError_t int8_allow_lds() {
+    const std::pair<void (*)(Int8Args), size_t> large[] = {{int8_direct_kernel<2, 2>, 8 * 16384},
+                                                           {int8_wide_kernel<4, 2, 3>, Wide256x128::kLds}};
+    for (const auto& [kernel, lds] : large) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
 
 hipError_t launch_copy_f32(const float* from, float* to, uint64_t count, hipStream_t stream) {
     hipLaunchKernelGGL(copy_f32_kernel, dim3(uint32_t((count + 255) / 256)), dim3(256), 0, stream, from, to, count);

@@ -49,6 +49,9 @@ struct Int8Call {
 // the ABI; for I8 rows copied from `given`, or left alone where that is null).
 hipError_t launch_int8_stage(const OpRows& x, uint64_t rows, uint32_t input, const float* given, int8_t* blocks,
                              float* scales, hipStream_t stream);
+// Lets the kernels with more than 64 KiB of LDS have it, on the current device;
+// every preparation of weights calls it, so no launch has to.
+hipError_t int8_allow_lds();
 hipError_t launch_copy_f32(const float* from, float* to, uint64_t count, hipStream_t stream);
 // Rows of one pass (a launch holds fewer than 2^32 threads).
 uint64_t int8_pass_rows(uint64_t rows, uint32_t output);

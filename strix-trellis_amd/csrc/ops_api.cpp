@@ -411,9 +411,14 @@ strix_status strix_amd_int8_weights_prepare(strix_context c, const strix_amd_int
     auto* impl = new (std::nothrow) strix_amd_int8_weights_impl;
     if (!impl) return STRIX_ERROR_OUT_OF_MEMORY;
     const uint32_t input = uint32_t(w.width), output = uint32_t(w.rows);
+    hipError_t e = stx::int8_allow_lds();
+    if (e != hipSuccess) {
+        delete impl;
+        return status_of(e);
+    }
     const uint64_t padded = stx::int8_row_blocks(w.rows) * 16, blocks = stx::int8_block_bytes(w.rows, input);
     impl->bytes = blocks + (bias.size ? 2 : 1) * padded * 4;
-    hipError_t e = hipMalloc(&impl->base, impl->bytes);
+    e = hipMalloc(&impl->base, impl->bytes);
     if (e != hipSuccess) {
         delete impl;
         return status_of(e);

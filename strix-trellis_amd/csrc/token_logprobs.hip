@@ -144,23 +144,16 @@ __device__ __forceinline__ uint32_t cut(uint64_t* list, uint32_t count, uint32_t
 
 // Writes the row's results from its statistics, the tokens ahead of the given
 // one, and the sorted list of its first tokens.
-template <class T>
-__device__ __forceinline__ void finish(const Args& a, uint64_t row, const Stats& t, uint32_t ahead,
-                                       const uint64_t* list) {
+__device__ __forceinline__ void finish(const Args& a, uint64_t row, const Stats& t, uint32_t token, float given,
+                                       uint32_t ahead, const uint64_t* list) {
     const Answer r = answer_of(t);
     const float nan = __builtin_nanf("");
     auto log_p = [&](float x) { return a.scale * (x - t.m) - r.log_sum; };
     if (threadIdx.x == 0) {
         if (a.entropy) st_global(a.entropy + row, r.valid ? r.entropy : nan);
-        if (a.tokens) {
-            const int32_t id = ld_global(a.tokens + row);
-            const bool fine = r.valid && uint32_t(id) < a.vocab;
-            if (a.ranks) st_global(a.ranks + row, fine ? int32_t(ahead) : -1);
-            if (a.logprobs) {
-                const float x = fine ? float(ld_global(static_cast<const T*>(a.logits) + row * a.stride + id)) : 0.0f;
-                st_global(a.logprobs + row, fine ? log_p(x) : nan);
-            }
-        }
+        const bool fine = r.valid && token < a.vocab;
+        if (a.ranks) st_global(a.ranks + row, fine ? int32_t(ahead) : -1);
+        if (a.logprobs) st_global(a.logprobs + row, fine ? log_p(given) : nan);
     }
     for (uint32_t j = threadIdx.x; j < a.top; j += kThreads) {
         const uint64_t k = list[j];
@@ -227,10 +220,10 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(Args a) {
     const uint32_t v1 = a.vocab - v0 < a.split_length ? a.vocab : v0 + a.split_length;
     const T* x = static_cast<const T*>(a.logits) + row * a.stride;
     using B = Batch<T>;
+    const uint32_t token = a.tokens ? uint32_t(ld_global(a.tokens + row)) : ~0u;   // first: its logit's address
     B batch, next, later;   // two batches ahead: a round trip to memory takes longer than a batch
     batch.load(x, v0, v1);
     if (v0 + kBatch < v1) next.load(x, v0 + kBatch, v1);
-    const uint32_t token = a.tokens ? uint32_t(ld_global(a.tokens + row)) : ~0u;
     const float given = token < a.vocab ? float(ld_global(x + token)) : kInf;
     Stats t = kNothing;        // m is the wave's
     uint32_t ahead = 0;        // the wave's
@@ -384,7 +377,7 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(Args a) {
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) ahead += wave_ahead[i];
     if (a.splits == 1) {
-        finish<T>(a, row, t, ahead, list);
+        finish(a, row, t, token, given, ahead, list);
         return;
     }
     const uint64_t p = row * a.splits + split;
@@ -402,26 +395,66 @@ template <class T>
 __global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(Args a) {
     __shared__ __align__(16) uint64_t list[kList];
     const uint64_t row = blockIdx.x, p = row * a.splits;
-    const uint32_t tid = threadIdx.x, last = a.vocab - (a.splits - 1) * a.split_length;
+    __shared__ uint32_t list_end;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, last = a.vocab - (a.splits - 1) * a.split_length;
     const uint32_t keys = a.top ? (a.splits - 1) * a.top + (last < a.top ? last : a.top) : 0;
     const uint64_t* from = a.part_keys + p * a.top;
-    // the list in rounds, as many keys at a time as it holds
-    uint32_t count = keys < kList ? keys : kList, taken = count;
-    for (uint32_t i = tid; i < count; i += kThreads) list[i] = ld_global(from + i);
+    if (tid == 0) list_end = 0;
+    const uint32_t token = a.tokens ? uint32_t(ld_global(a.tokens + row)) : ~0u;
+    // the thread's keys and the statistics on their way together
+    constexpr int kMine = 2;
+    uint64_t mine[kMine];
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) mine[j] = tid + j * kThreads < keys ? ld_global(from + tid + j * kThreads) : 0;
+    const float given =
+        token < a.vocab ? float(ld_global(static_cast<const T*>(a.logits) + row * a.stride + token)) : 0.0f;
+    // At least `top` keys reach the last key of any whole split, and the least of
+    // the whole splits' k-th keys where k of each make `top`.
+    uint64_t most_last = 0, least_kth = ~uint64_t(0);
+    const uint32_t kth = a.top ? (a.top + a.splits - 2) / (a.splits - 1) - 1 : 0;
     Stats t = kNothing;
     float ahead = 0;   // whole numbers of a row's tokens: two halves, each exact in a float sum
     float ahead_high = 0;
-    for (uint32_t i = tid & 63; i < a.splits; i += 64) {
+    for (uint32_t i = lane; i < a.splits; i += 64) {
         const f32x4 o = ld_global(reinterpret_cast<const f32x4*>(a.part + (p + i) * 8));
         const uint32_t n = ld_global(reinterpret_cast<const uint32_t*>(a.part + (p + i) * 8 + 4));
+        if (a.top && i + 1 < a.splits) {
+            const uint64_t u = ld_global(from + i * a.top + a.top - 1), v = ld_global(from + i * a.top + kth);
+            most_last = u > most_last ? u : most_last;
+            least_kth = v < least_kth ? v : least_kth;
+        }
         join(t, {o[0], o[1], o[2], o[3]}, a.c);
         ahead += float(n & 0x3FFFu);
         ahead_high += float(n >> 14);
     }
     t = join_lanes(t, a.c);
     const uint32_t total = uint32_t(wave_sum(ahead)) + (uint32_t(wave_sum(ahead_high)) << 14);
-    __syncthreads();
     if (a.top) {
+#pragma unroll
+        for (int o = 32; o; o >>= 1) {
+            const uint64_t u = __shfl_xor(most_last, o), v = __shfl_xor(least_kth, o);
+            most_last = u > most_last ? u : most_last;
+            least_kth = v < least_kth ? v : least_kth;
+        }
+        const uint64_t bound = most_last > least_kth ? most_last : least_kth;
+        __syncthreads();
+        auto enter = [&](uint64_t k) {
+            if (k < bound) return;
+            const uint32_t slot = atomicAdd(&list_end, 1u);
+            if (slot < kList) list[slot] = k;
+        };
+#pragma unroll
+        for (int j = 0; j < kMine; ++j)
+            if (tid + j * kThreads < keys) enter(mine[j]);
+        for (uint32_t i = tid + kMine * kThreads; i < keys; i += kThreads) enter(ld_global(from + i));
+        __syncthreads();
+        uint32_t count = list_end, taken = keys;
+        if (count > kList) {   // the list in rounds, as many keys at a time as it holds
+            __syncthreads();
+            count = taken = kList;
+            for (uint32_t i = tid; i < kList; i += kThreads) list[i] = ld_global(from + i);
+            __syncthreads();
+        }
         count = cut(list, count, a.top);
         while (taken < keys) {
             const uint32_t n = keys - taken < kList - count ? keys - taken : kList - count;
@@ -431,7 +464,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(Args a) {
             taken += n;
         }
     }
-    finish<T>(a, row, t, total, list);
+    finish(a, row, t, token, given, total, list);
 }
 
 template <class T>

@@ -159,7 +159,7 @@ static void int8_contract(Env& e) {
     x = d;
     x.weights.data = &x;   // host memory
     CHECK(prepare(x) == kArg);
-    for (int at = 0; at < 2; ++at) {
+    for (int at = 0; at < 3; ++at) {
         fake::launch_fail_at = at;
         CHECK(prepare(d) == kBackend && fake::live.size() == live1);
     }
@@ -438,6 +438,22 @@ static void logprobs_contract(Env& e) {
 
 // Passes and splits cover every row and token within the kernels' limits.
 static void sizing() {
+    // every row and channel lies in a tile, and a pass's workspace serves every smaller one
+    for (uint64_t rows : {1ull, 2ull, 4ull, 5ull, 8ull, 9ull, 16ull, 17ull, 32ull, 33ull, 64ull, 65ull, 333ull, 2048ull, 65536ull})
+        for (uint32_t I : {1u, 1536u, 1537u, 5120u, 40000u, 131071u})
+            for (uint32_t N : {1u, 16u, 512u, 5120u, 12288u, 129280u}) {
+                const stx::Int8Plan p = stx::int8_plan(rows, I, N);
+                const uint64_t shape[][2] = {{0, 0}, {16, 16}, {32, 32}, {32, 64}, {64, 64}, {128, 128}, {256, 128}};
+                if (p.core == stx::kInt8Decode) {
+                    CHECK(rows <= 8 && rows * (stx::int8_k_blocks(I) * 64 + 64) <= stx::kInt8DecodeLds && !p.bytes);
+                    continue;
+                }
+                CHECK(p.n_tiles == (N + shape[p.core][0] - 1) / shape[p.core][0]);
+                CHECK(p.m_tiles == (rows + shape[p.core][1] - 1) / shape[p.core][1]);
+                CHECK(p.core != stx::kInt8Rows16 || p.m_tiles == 1);
+                CHECK(p.scales_at == stx::int8_block_bytes(rows, I) && p.bytes >= p.scales_at + rows * 4);
+                CHECK(stx::int8_workspace_bytes(rows, I, N) >= stx::int8_workspace_bytes(rows - 1, I, N));
+            }
     for (uint64_t rows : {1ull, 9ull, 127ull, 128ull, 5000ull, 1ull << 20, 1ull << 31})
         for (uint32_t N : {1u, 128u, 4096u, 129280u, 16777216u}) {
             const uint64_t pass = stx::int8_pass_rows(rows, N);
