@@ -30,14 +30,32 @@ __device__ __forceinline__ RowScale row_scale(float most) {
     return r;
 }
 __device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+// The largest magnitude of a lane's inputs.  Magnitudes of 16-bit floats are in
+// the order of their bits, so those go two to an operation without conversions.
 template <class T>
-__device__ __forceinline__ float most_of(float most, const Raw4<T>& x) {
-    float v[4];
-    x.to(v);
+struct Most {
+    float m = 0.0f;
+    __device__ __forceinline__ void look(const Raw4<T>& x) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) most = maximum(most, fabsf(v[i]));
-    return most;
-}
+        for (int i = 0; i < 4; ++i) m = maximum(m, fabsf(x.v[i]));
+    }
+    __device__ __forceinline__ float value() const { return m; }
+};
+template <class T>
+    requires(sizeof(T) == 2)
+struct Most<T> {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 m = 0;
+    __device__ __forceinline__ void look(const Raw4<T>& x) {
+        const u32x2 u = __builtin_bit_cast(u32x2, x.v) & 0x7FFF7FFFu;
+        const uint32_t lo = u[0], hi = u[1];
+        m = __builtin_elementwise_max(m, __builtin_elementwise_max(__builtin_bit_cast(u16x2, lo), __builtin_bit_cast(u16x2, hi)));
+    }
+    __device__ __forceinline__ float value() const {
+        const uint16_t most = m[0] > m[1] ? m[0] : m[1];
+        return float(__builtin_bit_cast(T, most));
+    }
+};
 
 // Four inputs as int8 in one word.  q = x / s to the nearest integer, ties to
 // even: t = x * inv + 1.5 2^23 rounds x * inv to an integer in its low mantissa
@@ -50,14 +68,13 @@ __device__ __forceinline__ uint32_t round4(const Raw4<T>& x, const RowScale& r) 
     constexpr float kMagic = 12582912.0f;
     float v[4], t[4], d[4];
     x.to(v);
-    bool tie = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         t[i] = __builtin_fmaf(v[i], r.inv, kMagic);
         d[i] = __builtin_fmaf(kMagic - t[i], r.s, v[i]);
-        tie |= fabsf(d[i]) >= r.half;
     }
-    if (__any(tie)) {
+    const float farthest = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3])));
+    if (__any(farthest >= r.half)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const bool odd = __builtin_bit_cast(uint32_t, t[i]) & 1;
@@ -122,15 +139,15 @@ __global__ __launch_bounds__(256) void int8_stage_kernel(const T* x, uint64_t st
         if (at_end) put(inside, word_of(end));
         if (given && threadIdx.x == 0) st_global(scales + row, ld_global(given + row));
     } else {
-        float most = 0.0f;
+        Most<T> of_lane;
         for (uint32_t c = c0; c < inside; c += kAtOnce * 1024) {
             load_some(c);
 #pragma unroll
             for (int j = 0; j < kAtOnce; ++j)
-                if (c + j * 1024 < inside) most = most_of(most, raw[j]);
+                if (c + j * 1024 < inside) of_lane.look(raw[j]);
         }
-        if (at_end) most = most_of(most, end);
-        most = wave_reduce(most, maximum);
+        if (at_end) of_lane.look(end);
+        const float most = wave_reduce(of_lane.value(), maximum);
         if (lane == 0) wave_most[w] = most;
         __syncthreads();
         const RowScale r = row_scale(maximum(maximum(wave_most[0], wave_most[1]), maximum(wave_most[2], wave_most[3])));
@@ -198,9 +215,19 @@ __device__ __forceinline__ void emit(const Int8Args& a, uint32_t m, uint32_t n, 
 // One launch: every workgroup rounds the rows itself, into LDS, while its
 // weights (16 channels) are on their way.  Eight waves; the waves split K and add
 // their sums in LDS.  M: rows, rounded up to a power of two; 8 / M waves round one
-// row.  A row's share of a lane stays in registers where it fits, else it is
-// read twice (from the caches).
-template <class T, int M>
+// row.  Bound by the weights' bytes where there are many channels (4096 -> 12288
+// one row 7.7 us, 6.5 TB/s) and by one chain of latencies, launch, row, rounding,
+// products, where there are few (4096^2 3.3 us).
+// U: K blocks of a wave's part, all in flight at once, and with them the row's
+// share of each lane, which stays in registers between the maximum and the
+// rounding.  Every block that a wave asks for and does not have costs issue slots
+// and registers, and so workgroups per compute unit: 4096 -> 12288 one / four rows
+// take 7.7 / 9.1 us with U = 8 for 8.5 / 10.0 with U = 10 (5120^2 the other way:
+// 4.2 with 10, 5.6 with 8, in two batches), 1152 -> 5120 3.2 with 4, 4.0 with 10.
+// LONG: parts of several batches of U; the row is read twice, from the caches.
+// Its loads have code of their own: loads that may or may not have been followed
+// by others are waited for as if they had been, here with all the weights.
+template <class T, int M, int U, bool LONG>
 __global__ __launch_bounds__(512, 4) void int8_decode_kernel(Int8Args a, const T* x, uint64_t stride, uint32_t input) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int G = 8 / M;                  // waves per row
@@ -209,7 +236,6 @@ __global__ __launch_bounds__(512, 4) void int8_decode_kernel(Int8Args a, const T
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t kbs = a.k_blocks, kb0 = kbs * w / 8, kb1 = kbs * (w + 1) / 8;
     const uint32_t pitch = kbs * 64 + 64;     // bytes of a row in LDS: rows 16 banks apart
-    constexpr int U = 10;
     u32x4 f[U];
     const auto wr = make_rsrc(a.w + uint64_t(blockIdx.x) * kbs * 1024, kb1 * 1024);
     // blocks kb .. kb + U - 1; past the wave's part they read zeros
@@ -232,7 +258,7 @@ __global__ __launch_bounds__(512, 4) void int8_decode_kernel(Int8Args a, const T
         // the wave's groups of 256 inputs: b0, b0 + step, ..; the last may reach past the end
         const uint32_t b0 = part_of * 256, inside = input / 256 * 256;
         const bool at_end = input > inside && inside >= b0 && (inside - b0) % step == 0;
-        constexpr int kHeld = M == 1 ? 4 : M == 2 ? 6 : M == 4 ? 10 : 6;
+        constexpr int kHeld = (U * M + 3) / 4;   // the row's groups of U K blocks a wave
         Raw4<T> raw[kHeld], end;
         auto load_some = [&](uint32_t b) {
 #pragma unroll
@@ -245,26 +271,32 @@ __global__ __launch_bounds__(512, 4) void int8_decode_kernel(Int8Args a, const T
         __builtin_amdgcn_sched_barrier(0);
         load_w(kb0);
         __builtin_amdgcn_sched_barrier(0);
+        auto each = [&](uint32_t b, auto&& use) __attribute__((always_inline)) {
+#pragma unroll
+            for (int c = 0; c < kHeld; ++c)
+                if (b + c * step < inside) use(b + c * step, raw[c]);
+        };
+        auto others = [&](uint32_t b, auto&& use) __attribute__((always_inline)) {
+            for (; b < inside; b += kHeld * step) {
+                load_some(b);
+                each(b, use);
+            }
+        };
         if constexpr (std::is_same_v<T, int8_t>) {
-            for (uint32_t b = b0; b < inside && live; b += kHeld * step) {
-                if (b != b0) load_some(b);
-#pragma unroll
-                for (int c = 0; c < kHeld; ++c)
-                    if (b + c * step < inside) put(b + c * step, word_of(raw[c]));
+            auto copy = [&](uint32_t b, const Raw4<T>& r) __attribute__((always_inline)) { put(b, word_of(r)); };
+            if (live) {
+                each(b0, copy);
+                if (LONG) others(b0 + kHeld * step, copy);
+                if (at_end) put(inside, word_of(end));
+                if (lane == 0 && part_of == 0) row_s[m] = ld_global(a.s + m);
             }
-            if (at_end && live) put(inside, word_of(end));
-            if (live && lane == 0 && part_of == 0) row_s[m] = ld_global(a.s + m);
         } else {
-            float most = 0.0f;
-            const bool held = inside <= kHeld * step;
-            for (uint32_t b = b0; b < inside; b += kHeld * step) {
-                if (b != b0) load_some(b);
-#pragma unroll
-                for (int c = 0; c < kHeld; ++c)
-                    if (b + c * step < inside) most = most_of(most, raw[c]);
-            }
-            if (at_end) most = most_of(most, end);
-            most = wave_reduce(most, maximum);
+            Most<T> of_lane;
+            auto look = [&](uint32_t, const Raw4<T>& r) __attribute__((always_inline)) { of_lane.look(r); };
+            each(b0, look);
+            if (LONG) others(b0 + kHeld * step, look);
+            if (at_end) of_lane.look(end);
+            float most = wave_reduce(of_lane.value(), maximum);
             if constexpr (G > 1) {
                 if (lane == 0) wave_most[w] = most;
                 __syncthreads();
@@ -272,14 +304,13 @@ __global__ __launch_bounds__(512, 4) void int8_decode_kernel(Int8Args a, const T
                 for (int i = 0; i < G; ++i) most = maximum(most, wave_most[m * G + i]);
             }
             const RowScale r = row_scale(most);
-            for (uint32_t b = b0; b < inside && live; b += kHeld * step) {
-                if (!held) load_some(b);
-#pragma unroll
-                for (int c = 0; c < kHeld; ++c)
-                    if (b + c * step < inside) put(b + c * step, round4(raw[c], r));
+            auto round = [&](uint32_t b, const Raw4<T>& x4) __attribute__((always_inline)) { put(b, round4(x4, r)); };
+            if (live) {
+                if (LONG) others(b0, round);
+                else each(b0, round);
+                if (at_end) put(inside, round4(end, r));
+                if (lane == 0 && part_of == 0) row_s[m] = r.fine ? r.s : __builtin_nanf("");
             }
-            if (at_end && live) put(inside, round4(end, r));
-            if (live && lane == 0 && part_of == 0) row_s[m] = r.fine ? r.s : __builtin_nanf("");
         }
     }
     __syncthreads();
@@ -297,7 +328,7 @@ __global__ __launch_bounds__(512, 4) void int8_decode_kernel(Int8Args a, const T
             acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, f[u]), q, acc, 0, 0, 0);
         }
         kb += U;
-        if (kb >= kb1) break;
+        if (!LONG || kb >= kb1) break;
         load_w(kb);
     }
     part[w][lane] = acc;
@@ -311,13 +342,13 @@ __global__ __launch_bounds__(512, 4) void int8_decode_kernel(Int8Args a, const T
 // ---- nine to sixteen rows ----
 // One workgroup per 16 channels; its eight waves split K and add their sums in
 // LDS.
+template <int U>
 __global__ __launch_bounds__(512) void int8_rows16_kernel(Int8Args a) {
     __shared__ i32x4 part[8][64];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t kb0 = a.k_blocks * w / 8, kb1 = a.k_blocks * (w + 1) / 8;
     const auto wr = make_rsrc(a.w + uint64_t(blockIdx.x) * a.k_blocks * 1024, kb1 * 1024);
     const auto xr = make_rsrc(a.x, kb1 * 1024);
-    constexpr int U = 10;
     i32x4 acc{};
     for (uint32_t kb = kb0; kb < kb1; kb += U) {
         u32x4 f[U], g[U];   // blocks past kb1 read zeros
@@ -594,10 +625,19 @@ hipError_t decode(const Int8Args& a, const OpRows& x, uint32_t input, hipStream_
                            static_cast<const T*>(x.data), x.stride, input);
         return hipGetLastError();
     };
-    if (a.rows <= 1) return go(int8_decode_kernel<T, 1>);
-    if (a.rows <= 2) return go(int8_decode_kernel<T, 2>);
-    if (a.rows <= 4) return go(int8_decode_kernel<T, 4>);
-    return go(int8_decode_kernel<T, 8>);
+    // U: K blocks of a wave, an eighth of all
+    auto go_rows = [&](auto rows) {
+        constexpr int M = decltype(rows)::value;
+        if (a.k_blocks <= 32) return go(int8_decode_kernel<T, M, 4, false>);
+        if (a.k_blocks <= 64) return go(int8_decode_kernel<T, M, 8, false>);
+        if (a.k_blocks <= 80) return go(int8_decode_kernel<T, M, 10, false>);
+        return go(int8_decode_kernel<T, M, 8, true>);
+    };
+    using std::integral_constant;
+    if (a.rows <= 1) return go_rows(integral_constant<int, 1>{});
+    if (a.rows <= 2) return go_rows(integral_constant<int, 2>{});
+    if (a.rows <= 4) return go_rows(integral_constant<int, 4>{});
+    return a.k_blocks <= 32 ? go(int8_decode_kernel<T, 8, 4, false>) : hipErrorInvalidValue;
 }
 
 template <class F>
@@ -643,7 +683,10 @@ hipError_t launch_pass(const Int8Layer& w, const Int8Call& call, hipStream_t str
     if (e != hipSuccess) return e;
     const uint32_t tiles = plan.n_tiles * plan.m_tiles, spread = (plan.n_tiles + 7) / 8 * 8 * plan.m_tiles;
     switch (plan.core) {
-        case kInt8Rows16: return launch_core(int8_rows16_kernel, tiles, 512, 0, a, stream);
+        case kInt8Rows16:
+            if (a.k_blocks <= 32) return launch_core(int8_rows16_kernel<4>, tiles, 512, 0, a, stream);
+            if (a.k_blocks <= 64 || a.k_blocks > 80) return launch_core(int8_rows16_kernel<8>, tiles, 512, 0, a, stream);
+            return launch_core(int8_rows16_kernel<10>, tiles, 512, 0, a, stream);
         case kInt8Direct32x32: return launch_core(int8_direct_kernel<1, 1>, spread, 512, 8 * 4096, a, stream);
         case kInt8Direct32x64: return launch_core(int8_direct_kernel<1, 2>, spread, 512, 8 * 8192, a, stream);
         case kInt8Direct64x64: return launch_core(int8_direct_kernel<2, 2>, spread, 512, 8 * 16384, a, stream);

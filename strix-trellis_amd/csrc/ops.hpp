@@ -23,7 +23,8 @@ struct OpRows {
 // of the 16x16x64 integer MFMA: block (rb, kb) is 1 KiB at
 // (rb * k_blocks + kb) * 1024, its 16 bytes at lane l = 16 * piece + row % 16
 // are inputs 64 kb + 16 piece + 0..15 of row 16 rb + row % 16.  Rows are
-// padded to whole 32-row pairs of blocks and inputs to 128, with zeros.
+// padded to whole 32-row pairs of blocks, whose other rows hold anything, and
+// inputs to 128, with zeros.
 constexpr uint32_t int8_k_blocks(uint64_t input) { return uint32_t((input + 127) / 128 * 2); }
 constexpr uint64_t int8_row_blocks(uint64_t rows) { return (rows + 31) / 32 * 2; }
 constexpr uint64_t int8_block_bytes(uint64_t rows, uint64_t input) {

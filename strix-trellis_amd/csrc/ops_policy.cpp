@@ -14,13 +14,14 @@ uint64_t int8_pass_rows(uint64_t rows, uint32_t output) {
 
 Int8Plan int8_plan(uint64_t rows, uint32_t input, uint32_t output) {
     Int8Plan p;
-    const uint64_t kbs = int8_k_blocks(input), groups = (uint64_t(output) + 15) / 16;
+    const uint64_t kbs = int8_k_blocks(input);
     // A few rows: every 16-channel workgroup rounds the rows itself, which saves a
     // launch but costs each of them the rows' reads.  Against the two launches:
-    // 5120^2 one / two rows 6.6 / 7.6 us for 9.5, 4096 -> 12288 four rows 11.2
-    // for 12.8, 1152 -> 5120 eight rows 5.5 for 7.2; but 5120^2 eight rows 12.1
-    // for 8.0, 5120 -> 129280 four rows 137 for 117 (one row 103 for 114).
-    const bool decode = rows == 1 || (rows <= 4 && rows * groups <= 4096) || (rows <= 8 && input <= 1536);
+    // 5120^2 one / two / four rows 4.2 / 4.9 / 6.1 us for 7.7, 5120 -> 129280 four
+    // rows 111 for 117, 8192^2 four rows 14.3 for 14.8, 2048 -> 8192 eight rows 5.1
+    // for 5.9; but 12288 -> 4096 three rows 14.0 for 13.5, 4096 -> 12288 eight rows
+    // 11.7 for 10.8.
+    const bool decode = rows <= 2 || (rows <= 4 && input <= 8192) || (rows <= 8 && input <= 2048);
     if (decode && rows * (kbs * 64 + 64) <= kInt8DecodeLds) return p;   // needs no workspace
     p.scales_at = int8_block_bytes(rows, input);
     p.bytes = (p.scales_at + rows * 4 + 255) & ~uint64_t(255);
