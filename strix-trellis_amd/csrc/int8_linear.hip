@@ -378,10 +378,14 @@ __global__ __launch_bounds__(512) void int8_rows16_kernel(Int8Args a) {
 // part with operands straight from the caches (both are in MFMA order, 1 KiB per
 // load), two batches of U blocks in flight and no barrier.  The sums meet in
 // LDS, [wave][row][channel] with 16-byte units at unit ^ row, and leave as whole
-// rows of the tile.
+// rows of the tile.  Bound by the caches' latency and rate, so what counts is how
+// many waves a compute unit holds: the two small tiles run with one block in flight
+// twice and few registers, four and two workgroups to a compute unit (5120^2 24 /
+// 48 rows 9.7 us in 32 x 32, 11.3 in 32 x 64; with 4 and 3 blocks, one workgroup
+// each, 11.6 and 12.6).  64 x 64 has the LDS of a compute unit to itself.
 template <int TN, int TM>
-__global__ __launch_bounds__(512, 2) void int8_direct_kernel(Int8Args a) {
-    constexpr int BN = 32 * TN, BM = 32 * TM, U = TN * TM == 1 ? 4 : TN * TM == 2 ? 3 : 2;
+__global__ __launch_bounds__(512, TN * TM == 1 ? 8 : TN * TM == 2 ? 4 : 2) void int8_direct_kernel(Int8Args a) {
+    constexpr int BN = 32 * TN, BM = 32 * TM, U = TN * TM <= 2 ? 1 : 2;
     constexpr int kUnits = BN / 4, kPlane = BM * BN * 4;
     extern __shared__ __align__(16) unsigned char smem[];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;

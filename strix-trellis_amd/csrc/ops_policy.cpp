@@ -35,18 +35,32 @@ Int8Plan int8_plan(uint64_t rows, uint32_t input, uint32_t output) {
         tile(kInt8Rows16, 16, 16);
         return p;
     }
-    // The smallest direct tile whose workgroups (one per compute unit at a time)
-    // fill one round: 5120^2 48 rows 12.1 us in 32 x 64 tiles, 16.3 in 32 x 32 (two
-    // rounds), 15.0 in 64 x 64; 4096 -> 12288 48 rows 16.8 in 64 x 64, 20.1 in 32
-    // x 64, 21.3 in 32 x 32.  Up to 32 rows one and a half rounds of the smallest
-    // are faster than one of the next (4096 -> 12288 14.2 us for 16.1).
-    if (rows <= 64) {
-        if (tile(kInt8Direct32x32, 32, 32) <= (rows <= 32 ? 384 : 256)) return p;
-        if (tile(kInt8Direct32x64, 32, 64) <= 256) return p;
+    // The tile with the least estimated time: a start, and for each round (tiles over
+    // 256 compute units, rounded up) a part that is fixed and one that grows with the
+    // K blocks.  The figures (us) are fitted to 9 layers, 1152 to 12288 inputs and
+    // 512 to 20480 channels, at 17 to 1024 rows: of 135 cases the choice is within 4 % of
+    // the fastest in 132, 14 % behind it at worst.  Small tiles fill the compute units with few rows and
+    // channels, large ones read less: 5120^2 96 / 192 / 512 rows 12.6 / 19.0 / 39.5 us
+    // in 32 x 32 tiles, 14.7 / 16.8 / 38.1 in 32 x 64, 14.7 / 15.8 / 39.7 in 64 x 64,
+    // 26.7 / 27.1 / 29.9 in 128 x 128.
+    const struct {
+        Int8Core core;
+        uint32_t channels, rows;
+        float start, round, per_block;
+    } tiles[] = {{kInt8Direct32x32, 32, 32, 2.2f, 0.35f, 0.036f},
+                 {kInt8Direct32x64, 32, 64, 1.8f, 1.3f, 0.046f},
+                 {kInt8Direct64x64, 64, 64, 1.5f, 3.5f, 0.08f},
+                 {kInt8Wide128x128, 128, 128, 5.5f, 0.0f, 0.215f}};
+    float least = 0;
+    int best = -1;
+    for (int i = 0; i < 4; ++i) {
+        const auto& t = tiles[i];
+        const uint64_t rounds = (tile(t.core, t.channels, t.rows) + 255) / 256;
+        const float us = t.start + float(rounds) * (t.round + t.per_block * float(kbs));
+        if (best < 0 || us < least) best = i, least = us;
     }
-    // Past one round, LDS tiles: 5120^2 192 / 512 rows 16.7 / 39.5 us direct, 26.0 /
-    // 29.9 in 128 x 128 tiles; 4096 -> 12288 256 rows 39.8 and 24.8.
-    if (tile(kInt8Direct64x64, 64, 64) <= 256) return p;
+    tile(tiles[best].core, tiles[best].channels, tiles[best].rows);
+    if (tiles[best].core != kInt8Wide128x128) return p;
     // The larger LDS tile where it still fills two rounds: 4096 -> 12288 2048 rows
     // 112 us in 128 x 128, 107 in 256 x 128; 1024 rows 61 and 66.
     if (tile(kInt8Wide256x128, 256, 128) < 640) tile(kInt8Wide128x128, 128, 128);
