@@ -1,10 +1,12 @@
 """Token log probabilities (strix_amd_token_logprobs) against the definition in 64 bits.
 
-Tolerances.  With u = 2^-24 and V logits: a weight e^(c d) is off by 2 u |c d| from its exponent and 4 u from
-exp2f; a thread adds V / 512 of them, the joins of 64 lanes, 8 waves and up to V / 8192 splits rescale and add with
-under 4 roundings each.  The weights' mean |c d| is at most ln V + 2 where they matter (farther ones weigh less
-than 1 / V).  So log sum is off by at most u (V / 512 + 4 (14 + V / 8192) + 2 ln V + 20) =: e, a log probability by
-e + 4 u of its magnitude, and the entropy by e (2 + ln V).  Whole numbers are exact.
+Tolerances.  With u = 2^-24 and V logits: a weight e^(c d) is off by 3 u |c d| from its exponent (the rounded d, c
+and product) and 4 u from exp2f; a thread adds V / 512 of them, the joins of 64 lanes, 8 waves and up to V / 8192
+splits rescale and add with under 4 roundings each.  The weights' mean |c d| is at most ln V + 2 where they matter
+(farther ones weigh less than 1 / V).  So log sum is off by at most u (V / 512 + 4 (14 + V / 8192) + 2 ln V + 20)
+=: e, a log probability by e + 4 u of its magnitude, and the entropy by e (2 + ln V): the third u |c d| is in the 4
+per level, since the twelve levels of lanes and waves add without rescaling, one rounding each, and leave 36 u.
+Whole numbers are exact.
 """
 import math
 
