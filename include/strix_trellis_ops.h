@@ -11,7 +11,9 @@
  * is called directly, or prepared once as a plan (validated at creation;
  * submission allocates, copies, synchronises and queries nothing, so it can
  * be captured into a graph).  Calls and submissions that share a workspace or
- * an output must be ordered by the caller.
+ * an output must be ordered by the caller.  Weights and plans hold their context
+ * (it is not destroyed before them), plans their weights; every buffer is the
+ * caller's and has to outlive the work on it, captured graphs included.
  */
 #ifndef STRIX_TRELLIS_OPS_H
 #define STRIX_TRELLIS_OPS_H
@@ -116,7 +118,8 @@ strix_status strix_amd_int8_linear_plan_create(strix_context context, const stri
  * is absent drops out: no block or no residual: that term is 0 (one of the
  * two is needed); no gate or channel_scale: 1; no bias: 0.  hidden and normed
  * are each optional, one is needed; normed needs pre_weight and the reverse.
- * n is computed from u in FP32, before u is rounded to the views' type.
+ * n is computed from u in FP32, before u is rounded to the views' type; squares are
+ * summed in FP32 (a row whose squares pass 3.4e38 together has norm(v) = 0).
  * All views have one type (F32, F16 or BF16) and one width, 1..32768; the
  * gate is [rows][width], [1][width], [rows][1] or [1][1].  Vectors are F32
  * [width].  hidden and normed may each be exactly the memory of block or of
@@ -163,6 +166,8 @@ strix_status strix_amd_block_norm_plan_create(strix_context context, const strix
  * the order, by id.  A row with no logit above -inf, with a NaN or with a
  * +inf has no distribution: its floats are NaN and its integers -1.  A token
  * outside 0..vocab-1 gives NaN and -1 for that row's logprobs and ranks alone.
+ * A row's results do not depend on the other rows; the last bits of its floats
+ * may depend on their number (the order of the sums does).
  * Each output is optional, at least one is needed; logprobs and ranks need
  * tokens.  0 <= top <= min(vocab, STRIX_AMD_MAX_TOP); top_ids and
  * top_logprobs need top > 0.  The workspace is 256-byte aligned. */

@@ -5,6 +5,15 @@
 // first load to the last store, so every element is read and written once and
 // outputs may take the place of the inputs.  Sums are FP32: a thread's
 // channels, then its wave's lanes, then the waves, in that order always.
+//
+// Many rows are bound by their bytes: 4096 x 5120 F32 with both norms takes 64.2 us,
+// 5.2 TB/s, the rate of a large copy.  Few rows are bound by one chain of
+// latencies, launch, loads, two to four sums over the workgroup, stores: one row 3.9
+// us, of which a launch that only reads is 3.5; 333 x 4099 F16 with every part 9.6 us
+// at 1.3 workgroups a compute unit.  So a row has as many threads as leave each two or
+// three groups of four channels (5120 at 512), and every load is ahead of the first
+// sum; reading the row a second time for the second norm instead of holding it
+// would cost another round trip.
 #include "ops_device.hpp"
 
 namespace stx {

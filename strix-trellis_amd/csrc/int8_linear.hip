@@ -339,9 +339,12 @@ __global__ __launch_bounds__(512, 4) void int8_decode_kernel(Int8Args a, const T
     emit(a, m, n, acc, row_s[m], channels_of(a, n));
 }
 
-// ---- nine to sixteen rows ----
+// ---- up to sixteen rows ----
 // One workgroup per 16 channels; its eight waves split K and add their sums in
-// LDS.
+// LDS.  U: K blocks of a wave in flight, as in the decode kernel.  Bound by the
+// weights' bytes behind one round trip (5120^2 7.3 us for 26 MB, and 2.7 for the
+// rounding); 32 x 32 tiles instead are 0.2 us faster there, 1.1 slower at 4096^2, 5.5
+// slower at 12288 -> 4096.
 template <int U>
 __global__ __launch_bounds__(512) void int8_rows16_kernel(Int8Args a) {
     __shared__ i32x4 part[8][64];
@@ -475,6 +478,14 @@ __global__ __launch_bounds__(512, TN * TM == 1 ? 8 : TN * TM == 2 ? 4 : 2) void 
 // read while the step before multiplies.  The barrier stands between a stage's
 // steps: behind it every wave has read the whole stage, so its buffer takes the
 // DMA of the stage kRing ahead, and the next stage has landed.
+//
+// 4096 -> 12288, 2048 F32 rows: 108-123 us on different cards with the rounding of
+// the rows (13), 2.0 POPS at 8192 rows.  What bounds it is the clock under the
+// matrix pipes' load: the same launch takes 80 us on zeros (3.0 POPS at 8192 rows) and
+// 112 on random bytes, the pipes are busy half the time at 1.6 GHz, and tiles of
+// 192 x 256, with three quarters of the traffic into LDS, run at the same 2.0 POPS
+// there and lose where the tiles are few.  Without the LDS reads 105 us for 110,
+// without the DMA 85.
 template <int TN, int TM, int RING>
 struct WideShape {
     static constexpr int kBN = 64 * TN, kBM = 64 * TM, kStage = (TN + TM) * 4096, kRing = RING;
