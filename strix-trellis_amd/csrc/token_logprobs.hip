@@ -122,10 +122,31 @@ struct Args {
 
 // Sorts the first `top` of list[0..count) to its front (largest first) and
 // returns how many there are.  All threads call it; ends with a barrier.
-// Ranks by counting (every key is distinct), eight keys of the list in flight
-// per step; keys past the count are 0, which is ahead of none.
+// Ranks by counting (every key is distinct).  Up to 64 keys, the usual cut of a
+// few tokens, are spread over all threads and take one LDS round trip (512 x
+// 129280 BF16, 20 tokens, 42.0 -> 40.1 us; 33 x 100277, 5 tokens, 12.7 -> 11.9); more
+// go a key or two to a thread, eight of the list in flight per step, and keys past
+// the count are 0, which is ahead of none.
 __device__ __forceinline__ uint32_t cut(uint64_t* list, uint32_t count, uint32_t top) {
     typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+    if (count <= kThreads / 8) {   // eight threads to a key, eight keys each
+        const uint32_t i = threadIdx.x >> 3, part = threadIdx.x & 7;
+        __syncthreads();
+        const uint64_t mine = list[i];
+        uint64_t k[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) k[j] = list[part + 8 * j];
+        uint32_t ahead = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ahead += part + 8 * j < count && k[j] > mine;
+        ahead += __builtin_amdgcn_update_dpp(0, ahead, 0xB1, 0xf, 0xf, true);    // quad_perm 1,0,3,2
+        ahead += __builtin_amdgcn_update_dpp(0, ahead, 0x4E, 0xf, 0xf, true);    // quad_perm 2,3,0,1
+        ahead += __builtin_amdgcn_update_dpp(0, ahead, 0x141, 0xf, 0xf, true);   // row_half_mirror
+        __syncthreads();
+        if (part == 0 && i < count && ahead < top) list[ahead] = mine;
+        __syncthreads();
+        return count < top ? count : top;
+    }
     const uint32_t i0 = threadIdx.x, i1 = threadIdx.x + kThreads, padded = (count + 7) & ~7u;
     if (count + i0 < padded) list[count + i0] = 0;
     __syncthreads();
@@ -244,7 +265,7 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(Args a) {
     uint32_t since = v0, cut_at = v0;   // the first batch since then, the batch behind which the next cut comes
     if (tid == 0) list_end = 0;
 
-    auto enter = [&](uint32_t b0, const float (&v)[kEach]) {
+    auto enter = [&](uint32_t b0, const float (&v)[kEach]) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
             if (!__any(v[e] >= reach)) continue;
