@@ -6,7 +6,8 @@
 namespace stx {
 
 uint64_t int8_pass_rows(uint64_t rows, uint32_t output) {
-    // 64 x 64 tiles of 512 threads: 2^22 of them, 2^16 rows at most
+    // 64 x 64 tiles of 512 threads: 2^22 of them, 2^16 rows at most (smaller tiles are
+    // taken only where they are few)
     const uint64_t n_tiles = (uint64_t(output) + 63) / 64, most = (uint64_t(1) << 22) / n_tiles;
     const uint64_t pass = 64 * (most < 1024 ? most : 1024);
     return rows < pass ? rows : pass;

@@ -30,8 +30,8 @@
 // 55 us with 8 tokens, rank and entropy, 4.8 TB/s; entropy alone 44 us, with 20
 // tokens 51, in BF16, half the bytes, 28 and 42 (an exponential and six other
 // operations for each logit).  Few rows take two launches, up to 512 workgroups of
-// whole batches and a join: one row 13.3 us (the splits 8, the join 5), 33 rows of
-// 100277 BF16 14.5.  A last-arrival join in one launch would trade the second
+// whole batches and a join: one row 13.1 us (the splits 8, the join 5), 33 rows of
+// 100277 BF16 13.9.  A last-arrival join in one launch would trade the second
 // launch, 1.5 us or so, for a coherent round trip of about 1 and need counters that are
 // zero at the start, which a caller's workspace is not.
 #include "ops_device.hpp"

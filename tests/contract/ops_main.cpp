@@ -460,6 +460,13 @@ static void sizing() {
             CHECK(pass >= 1 && pass <= rows && (pass == rows || pass % 128 == 0));
             CHECK((pass + 127) / 128 * ((uint64_t(N) + 127) / 128) * 256 < uint64_t(1) << 32);
             CHECK(stx::int8_row_blocks(pass) * 4 * 256 < uint64_t(1) << 32);
+            // a launch of any core the plan picks for any part of a pass holds fewer than 2^32 threads
+            for (uint32_t I : {1u, 64u, 4096u, 40000u, 131071u})
+                for (uint64_t part = 1; part <= pass; part = part < pass ? (part * 2 < pass ? part * 2 : pass) : pass + 1) {
+                    const stx::Int8Plan p = stx::int8_plan(part, I, N);
+                    const uint64_t spread = uint64_t(p.n_tiles + 7) / 8 * 8 * p.m_tiles;
+                    CHECK(p.core == stx::kInt8Decode || spread * 512 < uint64_t(1) << 32);
+                }
         }
     for (uint64_t rows : {1ull, 2ull, 7ull, 511ull, 512ull, 1ull << 30})
         for (uint32_t vocab : {1u, 8192u, 8193u, 129280u, 1000000u, 2147483647u}) {
