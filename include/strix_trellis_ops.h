@@ -64,7 +64,8 @@ strix_status strix_amd_op_plan_destroy(strix_amd_op_plan plan);
  * (exactly: the quotient itself is rounded once).  A row with an infinity or
  * a NaN gives NaN outputs in that row alone.  The integer sum is exact; the
  * rest is FP32, rounded once to the output's type, so a row's bits do not
- * depend on the other rows or on their number.
+ * depend on the other rows or on their number.  s t sum is infinite only where
+ * that product is past FP32's range itself, whatever s and t are.
  *
  * Weights are prepared from device memory: I8 with their scales, or F32, F16
  * or BF16 rounded per channel by the rule above (a channel with an infinity

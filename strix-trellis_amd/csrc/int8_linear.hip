@@ -189,15 +189,30 @@ __device__ __forceinline__ Channels channels_of(const Int8Args& a, uint32_t n) {
     return c;
 }
 
+// A token's scale as s * by, with `by` a power of two that comes last: the sum
+// (below 2^31) times s stays finite for every s, and in the normal range where
+// the scale itself is below it, so only the output's own range counts.  By is 1
+// for scales of 2^-126 to 2^96; above, sum * s is at least 2^64, so that no channel
+// scale takes it below the normal range.
+struct TokenScale {
+    float s, by;
+};
+__device__ __forceinline__ TokenScale token_scale(float s) {
+    const float a = fabsf(s);
+    const bool large = a >= 0x1p96f, small = a < 0x1p-126f;
+    return {s * (large ? 0x1p-32f : small ? 0x1p32f : 1.0f), large ? 0x1p32f : small ? 0x1p-32f : 1.0f};
+}
+
 template <class T>
 __device__ __forceinline__ void emit4(const Int8Args& a, uint32_t m, uint32_t n, i32x4 acc, float s,
                                       const Channels& c) {
     T* row = static_cast<T*>(a.y) + uint64_t(m) * a.y_stride;
     float v[4], old[4];
     if (a.beta != 0.0f) load4(static_cast<const T*>(row), n, a.output, false).to(old);
+    const TokenScale ts = token_scale(s);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        v[i] = float(acc[i]) * s * c.t[i];
+        v[i] = float(acc[i]) * ts.s * c.t[i] * ts.by;
         if (c.bias) v[i] += c.b[i];
         v[i] *= a.alpha;
         if (a.beta != 0.0f) v[i] += a.beta * old[i];
