@@ -178,7 +178,10 @@ __device__ __forceinline__ void finish(const Args& a, uint64_t row, const Stats&
                                        uint32_t ahead, const uint64_t* list) {
     const Answer r = answer_of(t);
     const float nan = __builtin_nanf("");
-    auto log_p = [&](float x) { return a.scale * (x - t.m) - r.log_sum; };
+    // half the distance: finite logits may be farther apart than FP32 holds, and a
+    // small scale brings that back into its range (the halves round nothing that counts)
+    const float two = 2.0f * a.scale, half_m = 0.5f * t.m;
+    auto log_p = [&](float x) { return two * __builtin_fmaf(0.5f, x, -half_m) - r.log_sum; };
     if (threadIdx.x == 0) {
         if (a.entropy) st_global(a.entropy + row, r.valid ? r.entropy : nan);
         const bool fine = r.valid && token < a.vocab;
