@@ -119,8 +119,8 @@ strix_status strix_amd_int8_linear_plan_create(strix_context context, const stri
  * is absent drops out: no block or no residual: that term is 0 (one of the
  * two is needed); no gate or channel_scale: 1; no bias: 0.  hidden and normed
  * are each optional, one is needed; normed needs pre_weight and the reverse.
- * n is computed from u in FP32, before u is rounded to the views' type; squares are
- * summed in FP32 (a row whose squares pass 3.4e38 together has norm(v) = 0).
+ * n is computed from u in FP32, before u is rounded to the views' type; sums are
+ * FP32, and those past its range are taken of the row times a power of two.
  * All views have one type (F32, F16 or BF16) and one width, 1..32768; the
  * gate is [rows][width], [1][width], [rows][1] or [1][1].  Vectors are F32
  * [width].  hidden and normed may each be exactly the memory of block or of

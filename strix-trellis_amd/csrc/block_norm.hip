@@ -57,25 +57,48 @@ struct Share {
 // v -> norm(v) * (offset + weight) + bias over the row.  Channels past the
 // width are 0 before and after.  A weight that is not there yet (`late`) is
 // loaded behind the sums' inputs, so it arrives while they are added up.
+//
+// Sums or squares past FP32's range are taken again of the values times a power
+// of two; every thread has the same sum, so the whole workgroup does, and rows in
+// range pay one comparison for each sum (4096 x 5120 F32 63.9 -> 64.1 us, BF16 rows with
+// a gate 1 %).  Only scalars differ behind it: scaling the values themselves took
+// 13 registers more, and 65.8 us.
+// A LAYER row whose sum reaches 2^103 goes on at 2^-20 of its size (32768 values
+// at most then add up to less than 2^124; below 2^103 no value minus the mean leaves
+// the range either).  Squares are taken of values times 2^-80, and the reciprocal
+// keeps 2^8 that the weights give back, since 1 / 2^128 is below the normal range.
+// Infinities and NaN come out as they would without.
 template <int THREADS, int C>
 __device__ __forceinline__ void normalise(float (&v)[C][4], const NormCall& a, Share<float, THREADS, C>& weight,
                                           const float* late, Share<float, THREADS, C>& bias, const float* with_bias,
                                           bool late_bias, float* slots) {
     const uint32_t width = a.width;
+    float eps = a.eps;
     if (late) weight.load(late, width);
     if (a.layer) {
-        float s = 0.0f;
+        float s = 0.0f, size = 1.0f;
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < 4; ++i) s += v[c][i];
-        const float mean = group_sum<THREADS>(s, slots) / float(width);
+        s = group_sum<THREADS>(s, slots);
+        if (!(fabsf(s) < 0x1p103f)) {
+            size = 0x1p-20f;
+            eps = fmaxf(eps * size * size, 0x1p-126f);   // beside such a row's deviations, if it has any, nothing
+            s = 0.0f;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s = __builtin_fmaf(v[c][i], size, s);
+            s = group_sum<THREADS>(s, slots + 32);
+        }
+        const float mean = s / float(width);
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t k = (c * THREADS + threadIdx.x) * 4 + i;
-                v[c][i] = c + 1 < C || k < width ? v[c][i] - mean : 0.0f;
+                v[c][i] = c + 1 < C || k < width ? __builtin_fmaf(v[c][i], size, -mean) : 0.0f;
             }
     }
     float s = 0.0f;
@@ -83,12 +106,25 @@ __device__ __forceinline__ void normalise(float (&v)[C][4], const NormCall& a, S
     for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int i = 0; i < 4; ++i) s = __builtin_fmaf(v[c][i], v[c][i], s);
-    s = group_sum<THREADS>(s, slots + 16) / float(width);
-    const float inv = 1.0f / sqrtf(s + a.eps);
+    s = group_sum<THREADS>(s, slots + 16);
+    float back = 1.0f, up = 1.0f;
+    if (!(s < __builtin_inff())) {
+        constexpr float kDown = 0x1p-80f;
+        eps = eps * kDown * kDown;
+        up = kDown * 0x1p8f;
+        back = 0x1p-8f;
+        s = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s = __builtin_fmaf(v[c][i] * kDown, v[c][i] * kDown, s);
+        s = group_sum<THREADS>(s, slots + 48);
+    }
+    const float inv = up / sqrtf(s / float(width) + eps), offset = a.weight_offset * back;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[c][i] = v[c][i] * inv * (a.weight_offset + weight.raw[c].v[i]);
+        for (int i = 0; i < 4; ++i) v[c][i] = v[c][i] * inv * __builtin_fmaf(weight.raw[c].v[i], back, offset);
     if (with_bias) {
         if (late_bias) bias.load(with_bias, width);
 #pragma unroll
@@ -106,7 +142,7 @@ __device__ __forceinline__ void normalise(float (&v)[C][4], const NormCall& a, S
 enum Loads { kLate, kEarly, kAll };
 template <class T, int THREADS, int C, Loads LOADS>
 __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormCall a) {
-    __shared__ float slots[64];
+    __shared__ float slots[128];
     const uint64_t row = blockIdx.x;
     const uint32_t width = a.width;
     auto at = [&](const OpRows& r) { return static_cast<const T*>(r.data) + row * r.stride; };
@@ -176,7 +212,7 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormCall a) {
     // channels past the width: 0 again, whatever a gate or a bias made of them
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[C - 1][i] = ((C - 1) * THREADS + threadIdx.x) * 4 + i < width ? v[C - 1][i] : 0.0f;
-    normalise<THREADS>(v, a, pre, EARLY ? nullptr : a.pre_weight, pre_bias, a.pre_bias, !ALL, slots + 32);
+    normalise<THREADS>(v, a, pre, EARLY ? nullptr : a.pre_weight, pre_bias, a.pre_bias, !ALL, slots + 64);
     store(a.normed);
 }
 
