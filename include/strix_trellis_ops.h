@@ -167,8 +167,9 @@ strix_status strix_amd_block_norm_plan_create(strix_context context, const strix
  * the order, by id.  A row with no logit above -inf, with a NaN or with a
  * +inf has no distribution: its floats are NaN and its integers -1.  A token
  * outside 0..vocab-1 gives NaN and -1 for that row's logprobs and ranks alone.
- * A row's results do not depend on the other rows; the last bits of its floats
- * may depend on their number (the order of the sums does).
+ * Sums and logarithms are FP32.  A row's results do not depend on the other rows;
+ * the last bits of its floats may depend on their number (the order of the sums
+ * does).
  * Each output is optional, at least one is needed; logprobs and ranks need
  * tokens.  0 <= top <= min(vocab, STRIX_AMD_MAX_TOP); top_ids and
  * top_logprobs need top > 0.  The workspace is 256-byte aligned. */

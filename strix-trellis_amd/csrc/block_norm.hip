@@ -6,11 +6,15 @@
 // outputs may take the place of the inputs.  Sums are FP32: a thread's
 // channels, then its wave's lanes, then the waves, in that order always.
 //
-// Many rows are bound by their bytes: 4096 x 5120 F32 with both norms takes 64.2 us,
-// 5.2 TB/s, the rate of a large copy.  Few rows are bound by one chain of
-// latencies, launch, loads, two to four sums over the workgroup, stores: one row 3.9
-// us, of which a launch that only reads is 3.5; 333 x 4099 F16 with every part 9.6 us
-// at 1.3 workgroups a compute unit.  So a row has as many threads as leave each two or
+// Many rows are bound by their bytes: 4096 x 5120 F32 with both norms takes 63.8 us,
+// 5.3 TB/s, the rate of a large copy; in BF16, half the bytes, 42 us, 4.0 TB/s, so there
+// the chain of a row's latencies counts as well.  512 rows of 16384 F32 29.4 us, 4.6 TB/s;
+// of 32768 63 us, 4.3 TB/s (the F32 instance above 28672 channels spills 16 registers).  Few
+// rows are bound by one chain of latencies, launch, loads, two to four sums over the
+// workgroup, stores: one row 4.0 us, of which a launch that copies it is 2.9; 333 x 4099
+// F16 6.3 us with the two sums of RMS, 7.9 with the four of LAYER, 9.7 with gate, biases and
+// channel scale, at 1.3 workgroups a compute unit (8.7 at 4096 channels, without a third
+// group for three of them).  So a row has as many threads as leave each two or
 // three groups of four channels (5120 at 512), and every load is ahead of the first
 // sum; reading the row a second time for the second norm instead of holding it
 // would cost another round trip.

@@ -232,7 +232,9 @@ __device__ __forceinline__ void emit(const Int8Args& a, uint32_t m, uint32_t n, 
 // their sums in LDS.  M: rows, rounded up to a power of two; 8 / M waves round one
 // row.  Bound by the weights' bytes where there are many channels (4096 -> 12288
 // one row 7.7 us, 6.5 TB/s) and by one chain of latencies, launch, row, rounding,
-// products, where there are few (4096^2 3.3 us).
+// products, where there are few (4096^2 3.4 us).  The figures of this note and of
+// the sizing rule are of one layer again and again, which the last-level cache holds
+// (but for 5120 -> 129280); three layers of 4096^2 in turn take 4.1 to 4.5 us each.
 // U: K blocks of a wave's part, all in flight at once, and with them the row's
 // share of each lane, which stays in registers between the maximum and the
 // rounding.  Every block that a wave asks for and does not have costs issue slots
@@ -494,13 +496,14 @@ __global__ __launch_bounds__(512, TN * TM == 1 ? 8 : TN * TM == 2 ? 4 : 2) void 
 // steps: behind it every wave has read the whole stage, so its buffer takes the
 // DMA of the stage kRing ahead, and the next stage has landed.
 //
-// 4096 -> 12288, 2048 F32 rows: 108-123 us on different cards with the rounding of
-// the rows (13), 2.0 POPS at 8192 rows.  What bounds it is the clock under the
-// matrix pipes' load: the same launch takes 80 us on zeros (3.0 POPS at 8192 rows) and
-// 112 on random bytes, the pipes are busy half the time at 1.6 GHz, and tiles of
-// 192 x 256, with three quarters of the traffic into LDS, run at the same 2.0 POPS
-// there and lose where the tiles are few.  Without the LDS reads 105 us for 110,
-// without the DMA 85.
+// 4096 -> 12288, 2048 F32 rows: 108-130 us on different cards with the rounding of
+// the rows (13), 2.0 POPS at 8192 rows.  Two things are seen to cost.  The clock under
+// the matrix pipes' load: the same launch takes 80 us on zeros (3.0 POPS at 8192 rows)
+// and 112 on random bytes, at 1.6 GHz.  And the feed: the pipes are busy half the cycles,
+// 85 us are left of 110 without the DMA (105 without the LDS reads), 189 MB are fetched
+// for 59, and the library's product, whose outputs are the sums as they are, is 10 %
+// faster on random bytes at 8192 rows.  Tiles of 192 x 256, with three quarters of the
+// traffic into LDS, run at the same 2.0 POPS there and lose where the tiles are few.
 template <int TN, int TM, int RING>
 struct WideShape {
     static constexpr int kBN = 64 * TN, kBM = 64 * TM, kStage = (TN + TM) * 4096, kRing = RING;

@@ -27,13 +27,16 @@
 // (rising or equal logits) is filled again from memory, with a higher bound.
 //
 // Many rows are bound by their bytes and by what a logit costs: 512 x 129280 F32
-// 55 us with 8 tokens, rank and entropy, 4.8 TB/s; entropy alone 44 us, with 20
-// tokens 51, in BF16, half the bytes, 28 and 42 (an exponential and six other
-// operations for each logit).  Few rows take two launches, up to 512 workgroups of
-// whole batches and a join: one row 13.1 us (the splits 8, the join 5), 33 rows of
-// 100277 BF16 13.9.  A last-arrival join in one launch would trade the second
-// launch, 1.5 us or so, for a coherent round trip of about 1 and need counters that are
-// zero at the start, which a caller's workspace is not.
+// 55.5 us with 8 tokens, rank and entropy, 4.8 TB/s; entropy alone 50 us, all with 20
+// tokens 57; in BF16, half the bytes, 31 and 49 (an exponential and six other
+// operations for each logit; the entropy's sum is always taken).  From 257 to 512 rows a
+// row is one workgroup, 512 of which the chip holds at once, so 257 / 400 / 512 rows take
+// 45 / 50 / 56 us and 513, with a second round, 78.  Few rows take two launches, up to 512
+// workgroups of whole batches and a join: one row 12.8 us (the splits 8, the join 4; 6.9
+// with the entropy alone), 33 rows of 100277 BF16, half masked, 13.7, with 98 % masked 21
+// (few threads hold a finite logit, so there is no first bound and the list overflows).  A last-arrival join in one launch would save the
+// second launch, but needs a coherent round trip and counters that are zero at the
+// start, which a caller's workspace is not; it was not built.
 #include "ops_device.hpp"
 
 namespace stx {
@@ -124,9 +127,10 @@ struct Args {
 // returns how many there are.  All threads call it; ends with a barrier.
 // Ranks by counting (every key is distinct).  Up to 64 keys, the usual cut of a
 // few tokens, are spread over all threads and take one LDS round trip (512 x
-// 129280 BF16, 20 tokens, 42.0 -> 40.1 us; 33 x 100277, 5 tokens, 12.7 -> 11.9); more
-// go a key or two to a thread, eight of the list in flight per step, and keys past
-// the count are 0, which is ahead of none.
+// 129280 BF16, 20 tokens, 42.0 -> 40.1 us; 33 x 100277, 5 tokens, 12.7 -> 11.9: tokens and
+// entropy of the same normal logits each time, from the last-level cache); more go a key
+// or two to a thread, eight of the list in flight per step, and keys past the count are
+// 0, which is ahead of none.
 __device__ __forceinline__ uint32_t cut(uint64_t* list, uint32_t count, uint32_t top) {
     typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
     if (count <= kThreads / 8) {   // eight threads to a key, eight keys each
