@@ -296,18 +296,26 @@ def alloc_workspace(nbytes, device, like=None):
 
 
 
-def _on_stream(t, stream):
-    """Tell torch's caching allocator that `t` is used on `stream` (when that is
-    not the current stream), so its memory is not reused before the work
-    enqueued there has finished.  DeviceArrays are freed by their owner."""
-    if _is_torch(t) and stream is not None and _is_torch(stream) and stream != _t().cuda.current_stream(t.device):
-        t.record_stream(stream)
-    return t
+def _on_stream(allocate, stream, like):
+    """`allocate()`, a workspace for work on `stream` with tensors like `like`, on that stream.
+
+    Torch's caching allocator hands a block out again as soon as its last owner is gone, while that owner's work may
+    still be enqueued on the stream that the block was allocated on: only work on the same stream comes behind it.  So
+    a workspace is allocated with the stream that uses it as the current one, and goes back to later work on that
+    stream.  DeviceArrays come from the HIP runtime, which frees them behind all work."""
+    if stream is None or not _is_torch(like):
+        return allocate()
+    cuda = _t().cuda
+    if not _is_torch(stream):
+        stream = (cuda.ExternalStream(stream.cuda_stream, device=like.device) if stream.cuda_stream
+                  else cuda.default_stream(like.device))
+    with cuda.stream(stream):
+        return allocate()
 
 
 def _call(fn, weights, x, y, alpha, beta, workspace, stream, rank):
     if workspace is None:
-        workspace = _on_stream(alloc_workspace(workspace_bytes(weights, x, y, rank), x.device, x), stream)
+        workspace = _on_stream(lambda: alloc_workspace(workspace_bytes(weights, x, y, rank), x.device, x), stream, x)
     d = matmul_desc(weights, x, y, alpha, beta, workspace, rank)
     abi.check(fn(weights.ctx.handle, C.byref(d), C.byref(stream_desc(stream))), fn.__name__)
     return y
@@ -334,7 +342,7 @@ class LinearPlan:
     def __init__(self, weights, x, y, alpha=1.0, beta=0.0, workspace=None, stream=None, operation="gemv"):
         self.lib = weights.lib
         if workspace is None:
-            workspace = _on_stream(alloc_workspace(workspace_bytes(weights, x, y), x.device, x), stream)
+            workspace = _on_stream(lambda: alloc_workspace(workspace_bytes(weights, x, y), x.device, x), stream, x)
         self._keep = (weights, x, y, workspace)
         d = matmul_desc(weights, x, y, alpha, beta, workspace)
         op = abi.OPERATION_GEMV if operation == "gemv" else abi.OPERATION_GEMM
@@ -382,7 +390,7 @@ class GroupedGemvPlan:
         abi.check(self.lib.strix_grouped_gemv_workspace_bytes(ctx.handle, C.byref(d), C.byref(need)),
                   "strix_grouped_gemv_workspace_bytes")
         if workspace is None:
-            workspace = _on_stream(alloc_workspace(need.value, x.device), stream)
+            workspace = _on_stream(lambda: alloc_workspace(need.value, x.device), stream, x)
         d.workspace = C.c_void_p(workspace.data_ptr())
         d.workspace_bytes = workspace.numel()
         self._keep = (weights_list, x, y, workspace, handles)
@@ -483,7 +491,8 @@ class MoePlan:
                                                                            C.byref(need)),
                           "strix_amd_tp_moe_device_workspace_bytes")
         if workspace is None:
-            workspace = _on_stream(torch.empty(need.value // 4, dtype=torch.float32, device=x.device), stream)
+            workspace = _on_stream(lambda: torch.empty(need.value // 4, dtype=torch.float32, device=x.device),
+                                   stream, x)
         d.workspace = C.c_void_p(workspace.data_ptr())
         d.workspace_bytes = workspace.numel() * workspace.element_size()
         keep.append(workspace)
@@ -744,7 +753,7 @@ def _int8_desc(weights, x, y, x_scales, alpha, beta, workspace, stream):
                    output=op_view(y), alpha=alpha, beta=beta)
     if workspace is None:
         need = _query_workspace(weights.ctx, weights.lib.strix_amd_int8_linear_workspace_bytes, d)
-        workspace = _on_stream(alloc_workspace(need, x.device, x), stream)
+        workspace = _on_stream(lambda: alloc_workspace(need, x.device, x), stream, x)
     d.workspace = abi.Buffer(workspace.data_ptr() or None, workspace.numel() * workspace.element_size())
     return d, workspace
 
@@ -831,7 +840,7 @@ def _logprobs_desc(ctx, logits, tokens, logprobs, ranks, entropy, top_ids, top_l
                    top_ids=op_buffer(top_ids, "int32"), top_logprobs=op_buffer(top_logprobs), top=top, scale=scale)
     if workspace is None:
         need = _query_workspace(ctx, ctx.lib.strix_amd_token_logprobs_workspace_bytes, d)
-        workspace = _on_stream(alloc_workspace(need, logits.device, logits), stream)
+        workspace = _on_stream(lambda: alloc_workspace(need, logits.device, logits), stream, logits)
     d.workspace = abi.Buffer(workspace.data_ptr() or None, workspace.numel() * workspace.element_size())
     return d, workspace
 
