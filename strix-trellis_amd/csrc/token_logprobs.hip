@@ -34,9 +34,10 @@
 // 45 / 50 / 56 us and 513, with a second round, 78.  Few rows take two launches, up to 512
 // workgroups of whole batches and a join: one row 12.8 us (the splits 8, the join 4; 6.9
 // with the entropy alone), 33 rows of 100277 BF16, half masked, 13.7, with 98 % masked 21
-// (few threads hold a finite logit, so there is no first bound and the list overflows).  A last-arrival join in one launch would save the
-// second launch, but needs a coherent round trip and counters that are zero at the
-// start, which a caller's workspace is not; it was not built.
+// (few threads hold a finite logit, so there is no first bound and the list overflows).
+// A last-arrival join in one launch would save the second launch, but needs a coherent
+// round trip and counters that are zero at the start, which a caller's workspace is not;
+// it was not built.
 #include "ops_device.hpp"
 
 namespace stx {
