@@ -39,18 +39,6 @@ __device__ __forceinline__ float group_sum(float v, float* slot) {
     return v;
 }
 
-// 1 / (1 + e^-g), from e^-|g|, which does not overflow: e^-g does below -88, where the
-// gate is not 0 yet (it is below -104).  e^x = 2^n 2^r with n the integer nearest x log2 e,
-// log2 e in two parts, and n bounded where 2^n is 0 already; infinities and NaN go
-// through r.  Four operations fewer than a general exponential, which pay for the two
-// signs: 2048 x 5120 BF16 with a gate 27.9 us, 28.5 with expf.
-__device__ __forceinline__ float sigmoid(float g) {
-    constexpr float kLog2e = 1.44269504088896340736f, kRest = 1.92596299112661746887e-8f;
-    const float x = -fabsf(g), n = __builtin_rintf(fmaxf(x, -160.0f) * kLog2e);
-    const float r = __builtin_fmaf(x, kRest, __builtin_fmaf(x, kLog2e, -n));
-    const float e = __builtin_ldexpf(__builtin_amdgcn_exp2f(r), int(n));
-    return (g < 0.0f ? e : 1.0f) * __builtin_amdgcn_rcpf(1.0f + e);
-}
 
 // A thread's share of a row (or of a vector): groups of four channels, the
 // workgroup's groups side by side.  Every group but the last lies inside the

@@ -1,20 +1,8 @@
 // Operators around the trellis layers (include/strix_trellis_ops.h): argument
 // checks, the int8 weights, and prepared operators.
-//
-// Each operator is described by one function, which checks the descriptor and
-// the device residence of every buffer and leaves the kernels' arguments; a
-// direct call launches with them, a plan keeps them.  The order of the checks
-// is the linear calls': device, stream, descriptor, shapes and types,
-// overlaps, residence.
-#include <climits>
-#include <cmath>
-#include <new>
+#include "ops_internal.hpp"
 
-#include "api_internal.hpp"
-#include "ops.hpp"
-#include "strix_trellis_ops.h"
-
-using namespace stx_api;
+using namespace stx_ops;
 
 struct strix_amd_int8_weights_impl {
     strix_context owner = nullptr;
@@ -25,118 +13,6 @@ struct strix_amd_int8_weights_impl {
 };
 
 namespace {
-
-enum class Op { kInt8, kNorm, kLogprobs };
-
-}  // namespace
-
-// A plan counts among its context's live handles (strix_context_impl::weights_live).
-struct strix_amd_op_plan_impl {
-    strix_context owner = nullptr;
-    hipStream_t stream{};
-    Op op = Op::kInt8;
-    strix_amd_int8_weights weights = nullptr;
-    stx::Int8Call int8{};
-    stx::NormCall norm{};
-    uint32_t norm_type = 0;
-    stx::LogprobsCall logprobs{};
-};
-
-namespace {
-
-uint64_t size_of(uint32_t type) {
-    return type == stx::kF32 ? 4 : type == stx::kF16 || type == stx::kBF16 ? 2 : type == stx::kI8 ? 1 : 0;
-}
-bool is_float(uint32_t type) { return type == stx::kF32 || type == stx::kF16 || type == stx::kBF16; }
-
-// A view of the descriptor and the bytes it covers.
-struct Rows {
-    bool given = false;
-    uint64_t rows = 0, width = 0;
-    stx::OpRows at{};
-    Span span;
-    uint64_t align = 1;
-};
-
-bool absent(const strix_amd_view& v) {
-    static const strix_amd_view none{};
-    return std::memcmp(&v, &none, sizeof(v)) == 0;
-}
-
-strix_status read_view(const strix_amd_view& v, bool optional, Rows& out) {
-    out = {};
-    if (optional && absent(v)) return STRIX_SUCCESS;
-    const uint64_t size = size_of(v.dtype);
-    uint64_t last = 0, elements = 0, bytes = 0;
-    Rules r;
-    r.then([&] { return versioned(&v); })
-        .need(!v.flags, STRIX_ERROR_INVALID_ARGUMENT)
-        .need(size && v.rows <= INT_MAX && v.width >= 1 && v.width <= INT_MAX, STRIX_ERROR_UNSUPPORTED_FORMAT);
-    if (!r.held()) return r.status();
-    // row_stride counts only between rows
-    const uint64_t gaps = v.rows ? v.rows - 1 : 0;
-    r.need(!gaps || v.row_stride >= v.width, STRIX_ERROR_UNSUPPORTED_FORMAT)
-        .need(!v.rows || ((!gaps || checked_mul(gaps, v.row_stride, last)) &&
-                          !__builtin_add_overflow(last, v.width, &elements) && checked_mul(elements, size, bytes)),
-              STRIX_ERROR_INVALID_ARGUMENT);
-    if (!r.held()) return r.status();
-    out.given = true;
-    out.rows = v.rows;
-    out.width = v.width;
-    out.at = {v.data, v.rows > 1 ? v.row_stride : v.width, v.dtype};
-    out.span = Span(v.data, bytes);
-    out.align = size;
-    r.need(out.span.addressable(), STRIX_ERROR_INVALID_ARGUMENT)
-        .need(bytes <= v.buffer_bytes, STRIX_ERROR_INSUFFICIENT_BUFFER)
-        .need(!bytes || (v.data && out.span.aligned(size)), STRIX_ERROR_INVALID_ARGUMENT);
-    return r.status();
-}
-
-// A buffer of `count` 4-byte elements, or absent where that is allowed.
-strix_status read_buffer(const strix_amd_buffer& b, bool optional, uint64_t count, Span& out) {
-    out = {};
-    if (!b.data && !b.bytes && (optional || !count)) return STRIX_SUCCESS;
-    uint64_t bytes = 0;
-    Rules r;
-    r.need(checked_mul(count, 4, bytes), STRIX_ERROR_INVALID_ARGUMENT)
-        .need(b.bytes >= bytes, STRIX_ERROR_INSUFFICIENT_BUFFER);
-    if (!r.held()) return r.status();
-    out = Span(b.data, bytes);
-    r.need(b.data && out.addressable() && out.aligned(4), STRIX_ERROR_INVALID_ARGUMENT);
-    return r.status();
-}
-
-strix_status read_workspace(const strix_amd_buffer& b, uint64_t need, Span& out) {
-    out = Span(b.data, b.bytes);
-    Rules r;
-    r.need(b.bytes >= need, STRIX_ERROR_INSUFFICIENT_BUFFER)
-        .need(out.addressable() && (!b.bytes || (b.data && out.aligned(kWorkspaceAlign))),
-              STRIX_ERROR_INVALID_ARGUMENT);
-    return r.status();
-}
-
-bool apart(std::initializer_list<Span> written, std::initializer_list<Span> read) {
-    for (auto w = written.begin(); w != written.end(); ++w) {
-        for (auto v = w + 1; v != written.end(); ++v)
-            if (w->meets(*v)) return false;
-        for (const Span& v : read)
-            if (w->meets(v)) return false;
-    }
-    return true;
-}
-
-strix_status resident(strix_context c, std::initializer_list<Span> spans, uint64_t align) {
-    for (const Span& s : spans) {
-        const strix_status status = device_resident(c, s, align);
-        if (status != STRIX_SUCCESS) return status;
-    }
-    return STRIX_SUCCESS;
-}
-
-template <class T>
-T* at(const Span& s) {
-    return s.size ? static_cast<T*>(s.ptr()) : nullptr;
-}
 
 // ---- 8-bit integer linear ----
 
@@ -311,75 +187,41 @@ strix_status describe_logprobs(strix_context c, const strix_amd_token_logprobs_d
 
 // ---- calls and plans ----
 
-hipError_t launch(const strix_amd_op_plan_impl& p) {
-    switch (p.op) {
-        case Op::kInt8:
-            return p.int8.rows ? stx::launch_int8_linear(p.weights->layer, p.int8, p.stream) : hipSuccess;
-        case Op::kNorm: return p.norm.rows ? stx::launch_block_norm(p.norm, p.norm_type, p.stream) : hipSuccess;
-        case Op::kLogprobs:
-            return p.logprobs.rows ? stx::launch_token_logprobs(p.logprobs, p.stream) : hipSuccess;
+struct Int8Plan final : strix_amd_op_plan_impl {
+    strix_amd_int8_weights weights = nullptr;
+    stx::Int8Call call{};
+    strix_status describe(strix_context c, const strix_amd_int8_linear_desc* d) {
+        uint64_t need = 0;
+        const strix_status s = describe_int8(c, d, true, call, need);
+        if (s != STRIX_SUCCESS) return s;
+        weights = d->weights;
+        retained = &weights->plans;
+        return STRIX_SUCCESS;
     }
-    return hipErrorInvalidValue;
-}
-
-strix_status describe(strix_context c, const strix_amd_int8_linear_desc* d, strix_amd_op_plan_impl& p) {
-    uint64_t need = 0;
-    const strix_status s = describe_int8(c, d, true, p.int8, need);
-    if (s != STRIX_SUCCESS) return s;
-    p.op = Op::kInt8;
-    p.weights = d->weights;
-    return STRIX_SUCCESS;
-}
-strix_status describe(strix_context c, const strix_amd_block_norm_desc* d, strix_amd_op_plan_impl& p) {
-    p.op = Op::kNorm;
-    return describe_norm(c, d, p.norm, p.norm_type);
-}
-strix_status describe(strix_context c, const strix_amd_token_logprobs_desc* d, strix_amd_op_plan_impl& p) {
-    uint64_t need = 0;
-    p.op = Op::kLogprobs;
-    return describe_logprobs(c, d, true, p.logprobs, need);
-}
-
-template <class Desc>
-strix_status direct(strix_context c, const Desc* d, const strix_stream* stream) {
-    strix_amd_op_plan_impl p;
-    Rules r;
-    r.then([&] { return on_context_device(c); })
-        .then([&] { return borrowed_stream(c, stream, p.stream); })
-        .then([&] { return describe(c, d, p); })
-        .then([&] { return status_of(launch(p)); });
-    return r.status();
-}
-
-template <class Desc>
-strix_status create(strix_context c, const Desc* d, const strix_stream* stream, strix_amd_op_plan* out) {
-    if (!out) return STRIX_ERROR_INVALID_ARGUMENT;
-    *out = nullptr;
-    strix_amd_op_plan_impl p;
-    Rules r;
-    r.then([&] { return on_context_device(c); })
-        .then([&] { return borrowed_stream(c, stream, p.stream); })
-        .then([&] { return describe(c, d, p); });
-    if (!r.held()) return r.status();
-    p.owner = c;
-    auto* plan = new (std::nothrow) strix_amd_op_plan_impl(p);
-    if (!plan) return STRIX_ERROR_OUT_OF_MEMORY;
-    if (plan->weights) ++plan->weights->plans;
-    ++c->weights_live;
-    *out = plan;
-    return STRIX_SUCCESS;
-}
-
-template <class F>
-strix_status query(strix_context c, uint64_t* out, F&& describe) {
-    if (!out) return STRIX_ERROR_INVALID_ARGUMENT;
-    *out = 0;
-    uint64_t need = 0;
-    Rules r;
-    r.then([&] { return on_context_device(c); }).then([&] { return describe(need); });
-    if (r.held()) *out = need;
-    return r.status();
-}
+    hipError_t launch() const override {
+        return call.rows ? stx::launch_int8_linear(weights->layer, call, stream) : hipSuccess;
+    }
+};
+struct NormPlan final : strix_amd_op_plan_impl {
+    stx::NormCall call{};
+    uint32_t type = 0;
+    strix_status describe(strix_context c, const strix_amd_block_norm_desc* d) {
+        return describe_norm(c, d, call, type);
+    }
+    hipError_t launch() const override {
+        return call.rows ? stx::launch_block_norm(call, type, stream) : hipSuccess;
+    }
+};
+struct LogprobsPlan final : strix_amd_op_plan_impl {
+    stx::LogprobsCall call{};
+    strix_status describe(strix_context c, const strix_amd_token_logprobs_desc* d) {
+        uint64_t need = 0;
+        return describe_logprobs(c, d, true, call, need);
+    }
+    hipError_t launch() const override {
+        return call.rows ? stx::launch_token_logprobs(call, stream) : hipSuccess;
+    }
+};
 
 }  // namespace
 
@@ -460,21 +302,21 @@ strix_status strix_amd_int8_linear_workspace_bytes(strix_context c, const strix_
 }
 
 strix_status strix_amd_int8_linear(strix_context c, const strix_amd_int8_linear_desc* d, const strix_stream* stream) {
-    return direct(c, d, stream);
+    return direct<Int8Plan>(c, d, stream);
 }
 
 strix_status strix_amd_int8_linear_plan_create(strix_context c, const strix_amd_int8_linear_desc* d,
                                                const strix_stream* stream, strix_amd_op_plan* out) {
-    return create(c, d, stream, out);
+    return create<Int8Plan>(c, d, stream, out);
 }
 
 strix_status strix_amd_block_norm(strix_context c, const strix_amd_block_norm_desc* d, const strix_stream* stream) {
-    return direct(c, d, stream);
+    return direct<NormPlan>(c, d, stream);
 }
 
 strix_status strix_amd_block_norm_plan_create(strix_context c, const strix_amd_block_norm_desc* d,
                                               const strix_stream* stream, strix_amd_op_plan* out) {
-    return create(c, d, stream, out);
+    return create<NormPlan>(c, d, stream, out);
 }
 
 strix_status strix_amd_token_logprobs_workspace_bytes(strix_context c, const strix_amd_token_logprobs_desc* d,
@@ -485,23 +327,23 @@ strix_status strix_amd_token_logprobs_workspace_bytes(strix_context c, const str
 
 strix_status strix_amd_token_logprobs(strix_context c, const strix_amd_token_logprobs_desc* d,
                                       const strix_stream* stream) {
-    return direct(c, d, stream);
+    return direct<LogprobsPlan>(c, d, stream);
 }
 
 strix_status strix_amd_token_logprobs_plan_create(strix_context c, const strix_amd_token_logprobs_desc* d,
                                                   const strix_stream* stream, strix_amd_op_plan* out) {
-    return create(c, d, stream, out);
+    return create<LogprobsPlan>(c, d, stream, out);
 }
 
 strix_status strix_amd_op_plan_submit(strix_amd_op_plan p) {
     if (!p) return STRIX_ERROR_INVALID_ARGUMENT;
     const strix_status device = on_context_device(p->owner);
-    return device != STRIX_SUCCESS ? device : status_of(launch(*p));
+    return device != STRIX_SUCCESS ? device : status_of(p->launch());
 }
 
 strix_status strix_amd_op_plan_destroy(strix_amd_op_plan p) {
     if (!p) return STRIX_ERROR_INVALID_ARGUMENT;
-    if (p->weights) --p->weights->plans;
+    if (p->retained) --*p->retained;
     --p->owner->weights_live;
     delete p;
     return STRIX_SUCCESS;

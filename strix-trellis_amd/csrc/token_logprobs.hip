@@ -38,7 +38,7 @@
 // A last-arrival join in one launch would save the second launch, but needs a coherent
 // round trip and counters that are zero at the start, which a caller's workspace is not;
 // it was not built.
-#include "ops_device.hpp"
+#include "logprobs_device.hpp"
 
 namespace stx {
 
@@ -50,48 +50,11 @@ constexpr uint32_t kBatch = kThreads * kEach;
 static_assert(kBatch == kLogprobsBatch);
 constexpr uint32_t kList = 1024;                        // candidate capacity
 constexpr float kLn2 = 0.69314718055994530942f;
-constexpr float kLowest = -3.40282346638528859812e38f, kInf = __builtin_inff();
-
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t id) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);   // -0 counts as 0
-    return uint64_t(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | uint32_t(~id);
-}
-__device__ __forceinline__ float value_of(uint64_t key) {
-    const uint32_t b = uint32_t(key >> 32);
-    return __builtin_bit_cast(float, b & 0x80000000u ? b & 0x7FFFFFFFu : ~b);
-}
-__device__ __forceinline__ uint32_t id_of(uint64_t key) { return ~uint32_t(key); }
 
 // The next float above x (x not NaN or +inf).
 __device__ __forceinline__ float above(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
     return __builtin_bit_cast(float, b & 0x80000000u ? b - 1 : b + 1);
-}
-
-struct Stats {
-    float m, n, s, h;
-};
-constexpr Stats kNothing = {kLowest, 0.0f, 0.0f, 0.0f};
-
-// Distances past 2^24 have no weight at any admitted scale (2^24 times 2^-16
-// log2 e is over 300); kept finite, a weight of 0 times one is 0.
-__device__ __forceinline__ float power(float d, float c) { return fmaxf(d, -0x1p24f) * c; }
-
-// Statistics p against the larger maximum m.
-__device__ __forceinline__ Stats against(const Stats& p, float m, float c) {
-    const float d = power(p.m - m, c), f = __builtin_amdgcn_exp2f(d), t = p.n + p.s;
-    return p.m == m ? p : Stats{m, 0.0f, f * t, f * __builtin_fmaf(t, d, p.h)};
-}
-__device__ __forceinline__ void join(Stats& a, const Stats& b, float c) {
-    const float m = fmaxf(a.m, b.m);
-    const Stats x = against(a, m, c), y = against(b, m, c);
-    a = {m, x.n + y.n, x.s + y.s, x.h + y.h};
-}
-// Joins the lanes' statistics; every lane gets the result.
-__device__ __forceinline__ Stats join_lanes(const Stats& mine, float c) {
-    const float m = wave_max(mine.m);
-    const Stats x = against(mine, m, c);
-    return {m, wave_sum(x.n), wave_sum(x.s), wave_sum(x.h)};
 }
 
 // What the statistics of a whole row say; invalid rows give NaN.
@@ -122,6 +85,9 @@ struct Args {
     // ([rows][splits][8] words), then the keys ([rows][splits][top]).
     float* part;
     uint64_t* part_keys;
+    // PARTS: rows that are read (a finite score, not finished)
+    const float* scores;
+    const int32_t* finished;
 };
 
 // Sorts the first `top` of list[0..count) to its front (largest first) and
@@ -245,7 +211,8 @@ struct Batch {
     }
 };
 
-template <class T>
+// PARTS: the statistics and keys alone, of any number of splits, for another join.
+template <class T, bool PARTS>
 __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(Args a) {
     __shared__ __align__(16) uint64_t list[kList];
     __shared__ float wave_bound[kWaves];
@@ -257,6 +224,9 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(Args a) {
     const uint32_t split = blockIdx.x % a.splits, v0 = split * a.split_length;
     const uint32_t v1 = a.vocab - v0 < a.split_length ? a.vocab : v0 + a.split_length;
     const T* x = static_cast<const T*>(a.logits) + row * a.stride;
+    if constexpr (PARTS) {
+        if (!(fabsf(ld_global(a.scores + row)) < kInf) || (a.finished && ld_global(a.finished + row))) return;
+    }
     using B = Batch<T>;
     const uint32_t token = a.tokens ? uint32_t(ld_global(a.tokens + row)) : ~0u;   // first: its logit's address
     B batch, next, later;   // two batches ahead: a round trip to memory takes longer than a batch
@@ -414,7 +384,7 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(Args a) {
     ahead = 0;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) ahead += wave_ahead[i];
-    if (a.splits == 1) {
+    if (!PARTS && a.splits == 1) {
         finish(a, row, t, token, given, ahead, list);
         return;
     }
@@ -507,14 +477,55 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(Args a) {
 
 template <class T>
 hipError_t dispatch(const Args& a, uint64_t rows, hipStream_t stream) {
-    hipLaunchKernelGGL(token_logprobs_kernel<T>, dim3(a.splits * uint32_t(rows)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((token_logprobs_kernel<T, false>), dim3(a.splits * uint32_t(rows)), dim3(kThreads), 0, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
     hipLaunchKernelGGL(token_logprobs_join_kernel<T>, dim3(uint32_t(rows)), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
 
+template <class T>
+hipError_t dispatch_parts(const Args& a, uint64_t rows, hipStream_t stream) {
+    hipLaunchKernelGGL((token_logprobs_kernel<T, true>), dim3(a.splits * uint32_t(rows)), dim3(kThreads), 0, stream, a);
+    return hipGetLastError();
+}
+
 }  // namespace
+
+hipError_t launch_logprobs_parts(const OpRows& logits, uint64_t rows, uint32_t vocab, uint32_t top, float scale,
+                                 const float* scores, const int32_t* finished, void* workspace, hipStream_t stream) {
+    Args a{};
+    a.logits = logits.data;
+    a.stride = logits.stride;
+    a.vocab = vocab;
+    a.top = top;
+    a.scale = scale;
+    a.c = logprobs_exponent(scale);
+    a.splits = logprobs_splits(rows, vocab);
+    a.split_length = logprobs_split_length(a.splits, vocab);
+    a.part = static_cast<float*>(workspace);
+    a.part_keys = reinterpret_cast<uint64_t*>(a.part + rows * a.splits * 8);
+    a.scores = scores;
+    a.finished = finished;
+    constexpr uint64_t kRows = 1u << 20;   // a launch holds fewer than 2^32 threads
+    for (uint64_t left = rows; left;) {
+        const uint64_t n = left < kRows ? left : kRows;
+        hipError_t e = hipErrorInvalidValue;
+        switch (logits.type) {
+            case kF32: e = dispatch_parts<float>(a, n, stream); break;
+            case kF16: e = dispatch_parts<_Float16>(a, n, stream); break;
+            case kBF16: e = dispatch_parts<__bf16>(a, n, stream); break;
+        }
+        if (e != hipSuccess) return e;
+        left -= n;
+        a.logits = static_cast<const char*>(a.logits) + n * a.stride * (logits.type == kF32 ? 4 : 2);
+        a.scores += n;
+        if (a.finished) a.finished += n;
+        a.part += n * a.splits * 8;
+        a.part_keys += n * a.splits * top;
+    }
+    return hipSuccess;
+}
 
 hipError_t launch_token_logprobs(const LogprobsCall& call, hipStream_t stream) {
     Args a{};
@@ -529,10 +540,9 @@ hipError_t launch_token_logprobs(const LogprobsCall& call, hipStream_t stream) {
     a.vocab = call.vocab;
     a.top = call.top;
     a.scale = call.scale;
-    a.c = float(double(call.scale) * 1.4426950408889634074);
-    const uint64_t batches = (uint64_t(call.vocab) + kBatch - 1) / kBatch;
+    a.c = logprobs_exponent(call.scale);
     a.splits = logprobs_splits(call.rows, call.vocab);
-    a.split_length = uint32_t((batches + a.splits - 1) / a.splits) * kBatch;
+    a.split_length = logprobs_split_length(a.splits, call.vocab);
     a.part = static_cast<float*>(call.workspace);
     a.part_keys = reinterpret_cast<uint64_t*>(a.part + call.rows * a.splits * 8);
     // a launch holds fewer than 2^32 threads (more rows than that take one split)

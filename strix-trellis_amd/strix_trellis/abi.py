@@ -14,7 +14,7 @@ TRANSPORT_VERSION = 1
 WORKSPACE_ALIGNMENT = 256
 MARKER = {"3inst": 0, "mcg": 0xCBAC1FED, "mul1": 0x83DCD12D}
 CODEBOOK = {"3inst": 0, "mcg": 1, "mul1": 2}
-DTYPE_F16, DTYPE_BF16, DTYPE_F32, DTYPE_I8 = 1, 2, 3, 16
+DTYPE_F16, DTYPE_BF16, DTYPE_F32, DTYPE_I8, DTYPE_E4M3 = 1, 2, 3, 16, 17
 TRANSPORT_EXL3_CANONICAL = 1
 OPERATION_GEMV = 0
 OPERATION_GEMM = 1
@@ -161,6 +161,40 @@ class TokenLogprobsDesc(C.Structure):
                 ("top_logprobs", Buffer), ("top", u32), ("scale", f32), ("workspace", Buffer), ("reserved", u64 * 4)]
 
 
+class Fp8WeightsDesc(C.Structure):
+    _fields_ = [("struct_size", u32), ("abi_version", u32), ("weights", View), ("scales", Buffer), ("bias", Buffer),
+                ("up", View), ("up_scales", Buffer), ("up_bias", Buffer), ("reserved", u64 * 4)]
+
+
+class Fp8LinearDesc(C.Structure):
+    _fields_ = [("struct_size", u32), ("abi_version", u32), ("weights", vp), ("input", View),
+                ("input_scales", Buffer), ("output", View), ("alpha", f32), ("beta", f32), ("workspace", Buffer),
+                ("reserved", u64 * 4)]
+
+
+class Fp8GatedDesc(C.Structure):
+    _fields_ = [("struct_size", u32), ("abi_version", u32), ("weights", vp), ("input", View),
+                ("input_scales", Buffer), ("output", View), ("output_scales", Buffer), ("activation", u32),
+                ("flags", u32), ("workspace", Buffer), ("reserved", u64 * 4)]
+
+
+class BeamSelectDesc(C.Structure):
+    _fields_ = [("struct_size", u32), ("abi_version", u32), ("logits", View), ("scores", Buffer),
+                ("finished", Buffer), ("next_scores", Buffer), ("parents", Buffer), ("tokens", Buffer),
+                ("beams", u32), ("keep", u32), ("pad", i32), ("scale", f32), ("workspace", Buffer),
+                ("reserved", u64 * 4)]
+
+
+class States(C.Structure):
+    _fields_ = [("data", vp), ("buffer_bytes", u64), ("strides", u64 * 3)]
+
+
+class BeamReorderDesc(C.Structure):
+    _fields_ = [("struct_size", u32), ("abi_version", u32), ("parents", Buffer), ("source", States),
+                ("target", States), ("prompts", u64), ("outer", u64), ("inner", u64), ("bytes", u64),
+                ("beams", u32), ("flags", u32), ("reserved", u64 * 4)]
+
+
 def header(struct_type, **fields):
     """Zero-initialised descriptor with struct_size / abi_version set."""
     d = struct_type()
@@ -262,6 +296,19 @@ _PROTOTYPES = {
     "strix_amd_token_logprobs": (_S, [vp, C.POINTER(TokenLogprobsDesc), C.POINTER(Stream)]),
     "strix_amd_token_logprobs_plan_create": (_S, [vp, C.POINTER(TokenLogprobsDesc), C.POINTER(Stream),
                                                   C.POINTER(vp)]),
+    "strix_amd_fp8_weights_prepare": (_S, [vp, C.POINTER(Fp8WeightsDesc), C.POINTER(Stream), C.POINTER(vp)]),
+    "strix_amd_fp8_weights_destroy": (_S, [vp]),
+    "strix_amd_fp8_linear_workspace_bytes": (_S, [vp, C.POINTER(Fp8LinearDesc), C.POINTER(u64)]),
+    "strix_amd_fp8_linear": (_S, [vp, C.POINTER(Fp8LinearDesc), C.POINTER(Stream)]),
+    "strix_amd_fp8_linear_plan_create": (_S, [vp, C.POINTER(Fp8LinearDesc), C.POINTER(Stream), C.POINTER(vp)]),
+    "strix_amd_fp8_gated_workspace_bytes": (_S, [vp, C.POINTER(Fp8GatedDesc), C.POINTER(u64)]),
+    "strix_amd_fp8_gated": (_S, [vp, C.POINTER(Fp8GatedDesc), C.POINTER(Stream)]),
+    "strix_amd_fp8_gated_plan_create": (_S, [vp, C.POINTER(Fp8GatedDesc), C.POINTER(Stream), C.POINTER(vp)]),
+    "strix_amd_beam_select_workspace_bytes": (_S, [vp, C.POINTER(BeamSelectDesc), C.POINTER(u64)]),
+    "strix_amd_beam_select": (_S, [vp, C.POINTER(BeamSelectDesc), C.POINTER(Stream)]),
+    "strix_amd_beam_select_plan_create": (_S, [vp, C.POINTER(BeamSelectDesc), C.POINTER(Stream), C.POINTER(vp)]),
+    "strix_amd_beam_reorder": (_S, [vp, C.POINTER(BeamReorderDesc), C.POINTER(Stream)]),
+    "strix_amd_beam_reorder_plan_create": (_S, [vp, C.POINTER(BeamReorderDesc), C.POINTER(Stream), C.POINTER(vp)]),
 }
 
 GEMV_POLL_DEFAULT = 1 << 22

@@ -674,15 +674,19 @@ def _dtype_code(t):
             "int8": abi.DTYPE_I8}.get(name)
 
 
-def op_view(t):
+def op_view(t, e4m3=False):
     """strix_amd_view of a tensor [rows, width] (unit channel stride, any row stride); None: absent.
 
-    A width-1 column of a wider tensor passes as [rows, 1]."""
+    A width-1 column of a wider tensor passes as [rows, 1].  `e4m3`: of an operator that takes float8_e4m3fn (or its
+    bytes as uint8)."""
     if t is None:
         return abi.View()
     code = _dtype_code(t)
+    if e4m3 and str(t.dtype).split(".")[-1] in ("float8_e4m3fn", "uint8"):
+        code = abi.DTYPE_E4M3
     if code is None or t.dim() != 2:
-        raise ValueError("rows must be float32, float16, bfloat16 or int8 tensors [rows, width]")
+        raise ValueError("rows must be float32, float16, bfloat16 or " + ("float8_e4m3fn" if e4m3 else "int8") +
+                         " tensors [rows, width]")
     rows, width = int(t.shape[0]), int(t.shape[1])
     stride = t.stride(0) if _is_torch(t) else width
     if _is_torch(t) and width > 1 and t.stride(1) != 1:
@@ -866,3 +870,193 @@ class TokenLogprobsPlan(_OpPlan):
                                       workspace, stream)
         self._create(ctx, ctx.lib.strix_amd_token_logprobs_plan_create, d, stream,
                      (logits, tokens, logprobs, ranks, entropy, top_ids, top_logprobs, workspace))
+
+
+# ---------------------------------------------------------------------------
+# Layers in 8-bit floating point (include/strix_trellis_fp8.h)
+# ---------------------------------------------------------------------------
+
+
+class Fp8Weights:
+    """Weights of a layer in 8-bit floating point: `w` on the device, float8_e4m3fn [N, I] with `scales` float32
+    [ceil(N / 128), ceil(I / 128)], or a float32, float16 or bfloat16 [N, I] that is rounded per 128 x 128 block.
+    `bias` float32 [N] or None.  With `up` (and `up_scales`, `up_bias`) a pair for `fp8_gated`, `w` being the gate
+    projection.  (e4m3 may come as uint8, for hosts without torch.)"""
+
+    def __init__(self, ctx, w, scales=None, bias=None, up=None, up_scales=None, up_bias=None, stream=None):
+        self.ctx, self.lib = ctx, ctx.lib
+        self.output, self.input, self.pair = int(w.shape[0]), int(w.shape[1]), up is not None
+        d = abi.header(abi.Fp8WeightsDesc, weights=op_view(w, e4m3=True), scales=op_buffer(scales),
+                       bias=op_buffer(bias), up=op_view(up, e4m3=True), up_scales=op_buffer(up_scales),
+                       up_bias=op_buffer(up_bias))
+        h = C.c_void_p()
+        abi.check(self.lib.strix_amd_fp8_weights_prepare(ctx.handle, C.byref(d), C.byref(stream_desc(stream)),
+                                                         C.byref(h)), "strix_amd_fp8_weights_prepare")
+        self.handle = h
+
+    def destroy(self):
+        if self.handle:
+            abi.check(self.lib.strix_amd_fp8_weights_destroy(self.handle), "strix_amd_fp8_weights_destroy")
+            self.handle = None
+
+
+def _with_workspace(ctx, query, d, workspace, stream, like):
+    if workspace is None:
+        need = _query_workspace(ctx, query, d)
+        workspace = _on_stream(lambda: alloc_workspace(need, like.device, like), stream, like)
+    d.workspace = abi.Buffer(workspace.data_ptr() or None, workspace.numel() * workspace.element_size())
+    return d, workspace
+
+
+def _fp8_linear_desc(weights, x, y, x_scales, alpha, beta):
+    return abi.header(abi.Fp8LinearDesc, weights=weights.handle, input=op_view(x, e4m3=True),
+                      input_scales=op_buffer(x_scales), output=op_view(y), alpha=alpha, beta=beta)
+
+
+def fp8_linear_workspace_bytes(weights, x, y, x_scales=None):
+    return _query_workspace(weights.ctx, weights.lib.strix_amd_fp8_linear_workspace_bytes,
+                            _fp8_linear_desc(weights, x, y, x_scales, 1.0, 0.0))
+
+
+def fp8_linear(weights, x, y, x_scales=None, alpha=1.0, beta=0.0, workspace=None, stream=None):
+    """y = alpha * Fp8Linear(x) + beta * y: x [rows, I] float32, float16 or bfloat16 (rounded to e4m3 per row and block
+    of 128), or float8_e4m3fn with `x_scales` float32 [rows, ceil(I / 128)]; y [rows, N] float32, float16 or
+    bfloat16."""
+    d, workspace = _with_workspace(weights.ctx, weights.lib.strix_amd_fp8_linear_workspace_bytes,
+                                   _fp8_linear_desc(weights, x, y, x_scales, alpha, beta), workspace, stream, x)
+    abi.check(weights.lib.strix_amd_fp8_linear(weights.ctx.handle, C.byref(d), C.byref(stream_desc(stream))),
+              "strix_amd_fp8_linear")
+    return y
+
+
+class Fp8LinearPlan(_OpPlan):
+    """Prepared `fp8_linear` on fixed buffers."""
+
+    def __init__(self, weights, x, y, x_scales=None, alpha=1.0, beta=0.0, workspace=None, stream=None):
+        d, workspace = _with_workspace(weights.ctx, weights.lib.strix_amd_fp8_linear_workspace_bytes,
+                                       _fp8_linear_desc(weights, x, y, x_scales, alpha, beta), workspace, stream, x)
+        self._create(weights.ctx, weights.lib.strix_amd_fp8_linear_plan_create, d, stream,
+                     (weights, x, y, x_scales, workspace))
+
+
+GATED_ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def _fp8_gated_desc(weights, x, y, x_scales, y_scales, activation):
+    return abi.header(abi.Fp8GatedDesc, weights=weights.handle, input=op_view(x, e4m3=True),
+                      input_scales=op_buffer(x_scales), output=op_view(y, e4m3=True),
+                      output_scales=op_buffer(y_scales), activation=GATED_ACTIVATIONS[activation])
+
+
+def fp8_gated_workspace_bytes(weights, x, y, x_scales=None, y_scales=None, activation="silu"):
+    return _query_workspace(weights.ctx, weights.lib.strix_amd_fp8_gated_workspace_bytes,
+                            _fp8_gated_desc(weights, x, y, x_scales, y_scales, activation))
+
+
+def fp8_gated(weights, x, y, x_scales=None, y_scales=None, activation="silu", workspace=None, stream=None):
+    """The gated half of a feed-forward block, y = act(gate(x)) * up(x), on the pair `weights`: x as `fp8_linear` takes
+    it; y [rows, N] float32, float16 or bfloat16, or float8_e4m3fn with `y_scales` float32 [rows, ceil(N / 128)], as
+    the next `fp8_linear` takes it.  `activation`: "silu" or "gelu" (the tanh form)."""
+    d, workspace = _with_workspace(weights.ctx, weights.lib.strix_amd_fp8_gated_workspace_bytes,
+                                   _fp8_gated_desc(weights, x, y, x_scales, y_scales, activation), workspace, stream, x)
+    abi.check(weights.lib.strix_amd_fp8_gated(weights.ctx.handle, C.byref(d), C.byref(stream_desc(stream))),
+              "strix_amd_fp8_gated")
+    return y
+
+
+class Fp8GatedPlan(_OpPlan):
+    """Prepared `fp8_gated` on fixed buffers."""
+
+    def __init__(self, weights, x, y, x_scales=None, y_scales=None, activation="silu", workspace=None, stream=None):
+        d, workspace = _with_workspace(weights.ctx, weights.lib.strix_amd_fp8_gated_workspace_bytes,
+                                       _fp8_gated_desc(weights, x, y, x_scales, y_scales, activation), workspace,
+                                       stream, x)
+        self._create(weights.ctx, weights.lib.strix_amd_fp8_gated_plan_create, d, stream,
+                     (weights, x, y, x_scales, y_scales, workspace))
+
+
+# ---------------------------------------------------------------------------
+# Decoding with several beams (include/strix_trellis_beam.h)
+# ---------------------------------------------------------------------------
+
+
+def _beam_select_desc(logits, scores, next_scores, parents, tokens, beams, finished, pad, scale):
+    prompts = int(logits.shape[0]) // beams if beams > 0 else 0
+    for t in (next_scores, parents, tokens):
+        if t.dim() != 2 or int(t.shape[0]) != prompts or t.shape[1] != tokens.shape[1]:
+            raise ValueError("next_scores, parents and tokens must be [prompts, keep]")
+    return abi.header(abi.BeamSelectDesc, logits=op_view(logits), scores=op_buffer(scores),
+                      finished=op_buffer(finished, "int32"), next_scores=op_buffer(next_scores),
+                      parents=op_buffer(parents, "int32"), tokens=op_buffer(tokens, "int32"), beams=beams,
+                      keep=int(tokens.shape[1]), pad=pad, scale=scale)
+
+
+def beam_select(ctx, logits, scores, next_scores, parents, tokens, beams, finished=None, pad=0, scale=1.0,
+                workspace=None, stream=None):
+    """The best continuations of each prompt's beams: logits [prompts * beams, vocab], `scores` float32
+    [prompts * beams] (cumulative log probabilities; a beam at -inf offers nothing); `next_scores` float32, `parents`
+    (beams 0..beams-1) and `tokens` int32, all [prompts, keep], receive the `keep` largest of
+    scores + log softmax(scale * logits), equal ones by the lower beam, then the lower token.  A beam whose `finished`
+    (int32 [prompts * beams]) is not 0 offers the token `pad` alone, at its score.  Places that are left: -inf, -1, -1."""
+    d, workspace = _with_workspace(ctx, ctx.lib.strix_amd_beam_select_workspace_bytes,
+                                   _beam_select_desc(logits, scores, next_scores, parents, tokens, beams, finished, pad,
+                                                     scale), workspace, stream, logits)
+    abi.check(ctx.lib.strix_amd_beam_select(ctx.handle, C.byref(d), C.byref(stream_desc(stream))),
+              "strix_amd_beam_select")
+
+
+class BeamSelectPlan(_OpPlan):
+    """Prepared `beam_select` on fixed buffers."""
+
+    def __init__(self, ctx, logits, scores, next_scores, parents, tokens, beams, finished=None, pad=0, scale=1.0,
+                 workspace=None, stream=None):
+        d, workspace = _with_workspace(ctx, ctx.lib.strix_amd_beam_select_workspace_bytes,
+                                       _beam_select_desc(logits, scores, next_scores, parents, tokens, beams, finished,
+                                                         pad, scale), workspace, stream, logits)
+        self._create(ctx, ctx.lib.strix_amd_beam_select_plan_create, d, stream,
+                     (logits, scores, next_scores, parents, tokens, finished, workspace))
+
+
+def _states(t):
+    """strix_amd_states of a tensor [outer, rows, inner, width] with unit stride in its last dimension."""
+    if t.dim() != 4:
+        raise ValueError("states must be [outer, prompts * beams, inner, width]")
+    shape, size = [int(n) for n in t.shape], t.element_size()
+    if _is_torch(t):
+        if shape[3] > 1 and t.stride(3) != 1:
+            raise ValueError("states must have unit stride in their last dimension")
+        strides = [int(t.stride(i)) * size for i in range(3)]
+    else:
+        strides = [shape[1] * shape[2] * shape[3] * size, shape[2] * shape[3] * size, shape[3] * size]
+    extent = shape[3] * size + sum((n - 1) * s for n, s in zip(shape, strides)) if all(shape) else 0
+    return abi.States(t.data_ptr() or None, extent, (C.c_uint64 * 3)(*strides))
+
+
+def _beam_reorder_desc(parents, source, target):
+    if parents.dim() != 2 or tuple(source.shape) != tuple(target.shape) or source.dtype != target.dtype:
+        raise ValueError("parents must be [prompts, beams], and source and target of one shape and type")
+    prompts, beams = int(parents.shape[0]), int(parents.shape[1])
+    states = _states(source), _states(target)
+    if int(source.shape[1]) != prompts * beams:
+        raise ValueError("states must be [outer, prompts * beams, inner, width]")
+    return abi.header(abi.BeamReorderDesc, parents=op_buffer(parents, "int32"), source=states[0], target=states[1],
+                      prompts=prompts, beams=beams, outer=int(source.shape[0]), inner=int(source.shape[2]),
+                      bytes=int(source.shape[3]) * source.element_size())
+
+
+def beam_reorder(ctx, parents, source, target=None, stream=None):
+    """Row p * beams + b of `target` takes the contents of row p * beams + parents[p, b] of `source`: states of any type
+    [outer, prompts * beams, inner, width] (a cache [layers, rows, heads, length * size], say, or a slice of one up to
+    the length), `parents` int32 [prompts, beams].  A parent outside 0..beams-1 is the row itself.  No target, or the
+    source itself: in place, where rows that are their own parents are not touched."""
+    d = _beam_reorder_desc(parents, source, source if target is None else target)
+    abi.check(ctx.lib.strix_amd_beam_reorder(ctx.handle, C.byref(d), C.byref(stream_desc(stream))),
+              "strix_amd_beam_reorder")
+
+
+class BeamReorderPlan(_OpPlan):
+    """Prepared `beam_reorder` on fixed buffers."""
+
+    def __init__(self, ctx, parents, source, target=None, stream=None):
+        d = _beam_reorder_desc(parents, source, source if target is None else target)
+        self._create(ctx, ctx.lib.strix_amd_beam_reorder_plan_create, d, stream, (parents, source, target))
