@@ -21,10 +21,8 @@ constexpr uint64_t fp8_row_blocks(uint64_t rows) { return (rows + 31) / 32 * 2; 
 constexpr uint64_t fp8_block_bytes(uint64_t rows, uint64_t input) {
     return fp8_row_blocks(rows) * fp8_k_blocks(input) * 2048;
 }
-// Scales of rounded rows: [k_blocks][rows padded to 128], with the rows of each
-// 128 in the order that hands a lane those of rows r, r + 32, r + 64 and r + 96 at once.
-constexpr uint64_t fp8_padded_rows(uint64_t rows) { return (rows + 127) / 128 * 128; }
-constexpr uint32_t fp8_scale_at(uint32_t row) { return (row & ~127u) + (row & 31) * 4 + (row >> 5 & 3); }
+// Scales of rounded rows: [k_blocks][rows padded to 256].
+constexpr uint64_t fp8_padded_rows(uint64_t rows) { return (rows + 255) / 256 * 256; }
 
 // One layer, or a pair (the gate and up projections of one feed-forward block)
 // whose 32-row pairs of blocks alternate: gate channels 32 g + 0..31 in row
@@ -54,7 +52,7 @@ struct Fp8Call {
 // from the rule of the ABI).
 hipError_t launch_fp8_weights(const OpRows& w, uint64_t rows, uint32_t input, const float* given, uint8_t* blocks,
                               uint32_t step, float* scales, hipStream_t stream);
-// Rows of any type into blocks, with their scales in the order of fp8_scale_at.
+// Rows of any type into blocks, with their scales.
 hipError_t launch_fp8_rows(const OpRows& x, uint64_t rows, uint32_t input, const float* given, uint8_t* blocks,
                            float* scales, hipStream_t stream);
 // F32 rows to e4m3 rows with their scales.
@@ -67,18 +65,21 @@ hipError_t fp8_allow_lds();
 // How a pass of `rows` runs: its core, the core's tiles, and what lies where in
 // its workspace (the activations' blocks are at 0).
 enum Fp8Core : uint32_t {
-    kFp8Decode, kFp8Rows16, kFp8Direct32x32, kFp8Direct32x64, kFp8Direct64x32, kFp8Direct64x64,   // channels x rows
-    kFp8Wide128x128, kFp8Wide256x256
+    kFp8Decode,
+    kFp8Split16x16, kFp8Split16x32, kFp8Split32x16, kFp8Split32x32, kFp8Split32x64, kFp8Split64x64,
+    kFp8Wide128x128, kFp8Wide256x128, kFp8Wide256x256   // rows of weights x rows
 };
 struct Fp8Plan {
     Fp8Core core = kFp8Decode;
     uint32_t n_tiles = 0, m_tiles = 0;
-    uint64_t scales_at = 0, hidden_at = 0, bytes = 0;   // hidden: F32 rows that a second launch rounds to e4m3
+    uint64_t scales_at = 0, hidden_at = 0, bytes = 0;
+    bool hidden = false;   // F32 rows in the workspace that another launch rounds to e4m3
 };
 constexpr uint32_t kFp8DecodeLds = 44 * 1024;   // rows and scales of a decode launch in LDS
+// exact: products in FP32 whole (F32 and e4m3 outputs); rounded: e4m3 output.
 uint64_t fp8_pass_rows(uint64_t rows, uint32_t output);
-Fp8Plan fp8_plan(uint64_t rows, uint32_t input, uint32_t output, bool pair, bool rounded);
-uint64_t fp8_workspace_bytes(uint64_t rows, uint32_t input, uint32_t output, bool pair, bool rounded);
+Fp8Plan fp8_plan(uint64_t rows, uint32_t input, uint32_t output, bool pair, bool exact, bool rounded);
+uint64_t fp8_workspace_bytes(uint64_t rows, uint32_t input, uint32_t output, bool pair, bool exact, bool rounded);
 hipError_t launch_fp8(const Fp8Layer& w, const Fp8Call& call, hipStream_t stream);
 
 }  // namespace stx

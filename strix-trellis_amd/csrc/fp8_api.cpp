@@ -65,7 +65,7 @@ strix_status describe_rows(strix_context c, const Desc* d, bool pair, const stri
         .then([&] { return read_buffer(d->input_scales, !scaled, scaled ? x.rows * blocks_of(I) : 0, scales); })
         .then([&] { return read_buffer(output_scales, !rounded, rounded ? x.rows * blocks_of(N) : 0, out_scales); });
     if (!r.held()) return r.status();
-    need = x.rows ? stx::fp8_workspace_bytes(x.rows, uint32_t(I), uint32_t(N), pair, rounded) : 0;
+    need = x.rows ? stx::fp8_workspace_bytes(x.rows, uint32_t(I), uint32_t(N), pair, y.at.type == stx::kF32 || rounded, rounded) : 0;
     if (!place) return STRIX_SUCCESS;
     const Span held(w->base, w->bytes);
     r.then([&] { return read_workspace(d->workspace, need, workspace); })

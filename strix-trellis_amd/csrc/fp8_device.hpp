@@ -107,10 +107,16 @@ __device__ __forceinline__ f32x16 product32(const u32x4 (&w)[2][2], const u32x4 
     return p;
 }
 
+// A value that is the same for a whole wave and that no kernel running meanwhile writes:
+// a scalar load, which does not count among the vector loads in flight.
+__device__ __forceinline__ float ld_uniform(const float* p) {
+    return *(const __attribute__((address_space(4))) float*)(p);
+}
+
 struct Fp8Args {
     const uint8_t* w;         // blocks of weights
     const uint8_t* x;         // blocks of rows
-    const float *t, *s;       // scales of weights, of rows (in the order of fp8_scale_at, or given rows)
+    const float *t, *s;       // scales of weights, of rows ([k_blocks][s_pitch], or as given)
     const float* bias;        // null: none
     void* y;
     uint64_t y_stride;

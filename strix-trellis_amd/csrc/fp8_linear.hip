@@ -8,6 +8,7 @@
 #include <utility>
 
 #include "fp8_device.hpp"
+#include "fp8_wide.hpp"
 
 namespace stx {
 
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(512) void fp8_decode_kernel(Fp8Args a, const T* x, 
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 const f32x4 v = product16<true>(f[p][u], q);
-                const float st = s * ld_global(t[p] + kb + u);
+                const float st = s * ld_uniform(t[p] + kb + u);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[p][i] = __builtin_fmaf(v[i], st, acc[p][i]);
             }
@@ -119,171 +120,126 @@ __global__ __launch_bounds__(512) void fp8_decode_kernel(Fp8Args a, const T* x, 
     else emit(a, m, n, with_bias(a, n, acc[0]), true);
 }
 
-// ---- up to sixteen rows ----
-// One workgroup per 16 channels (of both projections in a pair); its eight waves
-// split K and add their sums in LDS.  U: blocks of a wave in flight.
-template <int U, bool PAIR>
-__global__ __launch_bounds__(512) void fp8_rows16_kernel(Fp8Args a) {
-    constexpr int P = PAIR ? 2 : 1;
-    __shared__ f32x4 part[P][8][64];
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const uint32_t kbs = a.k_blocks, kb0 = kbs * w / 8, kb1 = kbs * (w + 1) / 8, c = blockIdx.x;
-    const auto xr = make_rsrc(a.x, kb1 * 2048);
-    const auto gr = make_rsrc(a.w + uint64_t(PAIR ? c / 2 * 4 + c % 2 : c) * kbs * 2048, kb1 * 2048);
-    const auto ur = make_rsrc(a.w + uint64_t(c / 2 * 4 + c % 2 + 2) * kbs * 2048, kb1 * 2048);
-    const float* t[2] = {a.t + uint64_t(c / 8) * kbs, a.t + a.t_up + uint64_t(c / 8) * kbs};
-    const uint32_t m = lane & 15;
-    const float* s = a.s + fp8_scale_at(m);
-    f32x4 acc[P] = {};
-    for (uint32_t kb = kb0; kb < kb1; kb += U) {
-        u32x4 f[P][U][2], g[U][2];   // blocks past kb1 read zeros
-        float st[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t at = (kb + u) * 2048 + j * 1024 + lane * 16;
-                f[0][u][j] = __builtin_amdgcn_raw_buffer_load_b128(gr, at, 0, 0);
-                if (PAIR) f[P - 1][u][j] = __builtin_amdgcn_raw_buffer_load_b128(ur, at, 0, 0);
-            }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            st[u] = ld_global(s + uint64_t(kb + u < kb1 ? kb + u : kb1 - 1) * a.s_pitch);
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                g[u][j] = __builtin_amdgcn_raw_buffer_load_b128(xr, (kb + u) * 2048 + j * 1024 + lane * 16, 0, 0);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (kb + u >= kb1) break;
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
-                const f32x4 v = product16<true>(f[p][u], g[u]);
-                const float by = st[u] * ld_global(t[p] + kb + u);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[p][i] = __builtin_fmaf(v[i], by, acc[p][i]);
-            }
-        }
-    }
-#pragma unroll
-    for (int p = 0; p < P; ++p) part[p][w][lane] = acc[p];
-    __syncthreads();
-    const uint32_t n = c * 16 + 4 * (lane >> 4);
-    if (w || m >= a.rows || n >= a.output) return;
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-        for (int j = 1; j < 8; ++j) acc[p] += part[p][j][lane];
-    if constexpr (PAIR) emit(a, m, n, gated4(a, n, acc[0], acc[1]), false);
-    else emit(a, m, n, with_bias(a, n, acc[0]), true);
-}
-
-// ---- tens to hundreds of rows ----
-// Tiles of 32 TN rows of weights (a pair: 16 TN channels of either projection) x 32
-// TM rows, few and short: the tile's K is split over the workgroup's eight
-// waves, each of which multiplies the whole tile over its part with operands
-// straight from the caches (both are in MFMA order), two blocks in flight and no
+// ---- up to hundreds of rows ----
+// Tiles of 16 TN rows of weights (a pair: half of them of either projection) x 16 TM
+// rows, few and short: the tile's K is split over the workgroup's eight waves, each
+// of which multiplies the whole tile over its part with operands straight from the
+// caches (both are in MFMA order), two batches of U blocks in flight and no
 // barrier.  The sums meet in LDS, [wave][row][channel] with 16-byte units at
 // unit ^ row, and leave as whole rows of the tile.
-template <int TN, int TM, bool PAIR, bool EXACT>
-__global__ __launch_bounds__(512, TN * TM == 1 ? 4 : 2) void fp8_direct_kernel(Fp8Args a) {
-    static_assert(!PAIR || TN == 2);
-    constexpr int BN = 32 * TN, BM = 32 * TM;
-    constexpr int kUnits = BN / 4, kPlane = BM * BN * 4;
+template <int TN_, int TM_, int U_, int WAVES_>
+struct SplitShape {
+    static constexpr int TN = TN_, TM = TM_, U = U_, kUnits = 4 * TN, kPlane = 16 * TM * kUnits * 16;
+    static constexpr int kSimd = WAVES_;   // waves a SIMD holds
+    static constexpr size_t kLds = 8 * size_t(kPlane);
+};
+
+template <class S, bool PAIR, bool EXACT>
+__global__ __launch_bounds__(512, S::kSimd) void fp8_split_kernel(Fp8Args a) {
+    constexpr int TN = S::TN, TM = S::TM, U = S::U;
+    static_assert(!PAIR || TN % 2 == 0);
     extern __shared__ __align__(16) unsigned char smem[];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     // The row tiles of a channel tile run on one XCD (workgroup i on XCD i % 8), whose
     // L2 then reads the weights once.
     const uint32_t b = blockIdx.x / 8, nt = b / a.m_tiles * 8 + blockIdx.x % 8, mt = b % a.m_tiles;
     if (nt >= a.n_tiles) return;
-    const uint32_t kbs = a.k_blocks, kb0 = kbs * w / 8, kb1 = kbs * (w + 1) / 8, pair = kbs * 2048;
-    const uint32_t weight_rows = PAIR ? (a.output + 31) / 32 * 64 : a.output;
-    const uint32_t nb = (weight_rows + 31) / 32 * 2 - nt * 2 * TN, mb = (a.rows + 31) / 32 * 2 - mt * 2 * TM;
-    // blocks of channels or rows past the last read zeros
-    const auto wr = make_rsrc(a.w + uint64_t(nt) * 2 * TN * pair, (nb < 2 * TN ? nb : 2 * TN) * pair);
-    const auto xr = make_rsrc(a.x + uint64_t(mt) * 2 * TM * pair, (mb < 2 * TM ? mb : 2 * TM) * pair);
-    const int h = lane >> 5, r16 = lane & 15, hi = (lane >> 4) & 1;
-    const uint32_t piece = hi * pair + (2 * h * 16 + r16) * 16;
-    const float* s[TM];
+    const uint32_t kbs = a.k_blocks, kb0 = kbs * w / 8, kb1 = kbs * (w + 1) / 8, block_row = kbs * 2048;
+    // blocks of channels c, c + 1, ..; of a pair the first half are gates, the others their ups
+    constexpr int kTiles = PAIR ? TN / 2 : TN;
+    const uint32_t c0 = nt * kTiles, blocks = (a.output + 31) / 32 * 2;
+    // Uniform offsets of the operands' row blocks.  Blocks past the last repeat it (their sums
+    // go nowhere).
+    uint32_t w_at[TN], x_at[TM];
     const float* t[TN];
 #pragma unroll
-    for (int k = 0; k < TM; ++k) s[k] = a.s + fp8_scale_at(mt * BM + k * 32 + (lane & 31));
-#pragma unroll
     for (int i = 0; i < TN; ++i) {
-        // channels of a tile past the last have no scales of their own
-        const uint32_t n = PAIR ? nt * 32 : nt * BN + i * 32, block = (n < a.output ? n : 0) / 128;
-        t[i] = a.t + (PAIR && i ? a.t_up : 0) + uint64_t(block) * kbs;
+        const uint32_t c = c0 + i % kTiles < blocks ? c0 + i % kTiles : blocks - 1;
+        w_at[i] = (PAIR ? c / 2 * 4 + c % 2 + i / kTiles * 2 - c0 / 2 * 4 : c - c0) * block_row;
+        // tiles past the last have no scales of their own
+        t[i] = a.t + (PAIR && i >= kTiles ? a.t_up : 0) + uint64_t((c * 16 < a.output ? c : 0) / 8) * kbs;
     }
+    const uint32_t m_blocks = (a.rows + 15) / 16 - mt * TM;
+#pragma unroll
+    for (int k = 0; k < TM; ++k) x_at[k] = (uint32_t(k) < m_blocks ? k : m_blocks - 1) * block_row;
+    constexpr uint32_t kSpan = PAIR ? (TN + 3) / 4 * 4 : TN;
+    const auto wr = make_rsrc(a.w + uint64_t(PAIR ? c0 / 2 * 4 : c0) * block_row, kSpan * block_row);
+    const auto xr = make_rsrc(a.x + uint64_t(mt) * TM * block_row, TM * block_row);
+    const float* s = a.s + mt * 16 * TM + (lane & 15);
     struct Operands {
-        u32x4 f[TN][2][2], g[TM][2][2];
-        float s[TM];
+        u32x4 f[U][TN][2], g[U][TM][2];
+        float s[U][TM];
     };
     auto load = [&](Operands& o, uint32_t kb) {
-        const bool live = kb < kb1;   // past the wave's part: out of range, zeros
-        const uint32_t at = piece + (live ? kb * 2048 : 0x80000000u);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int u = 0; u < U; ++u) {
+            // past the wave's part: out of range, zeros
+            const bool live = kb + u < kb1;
+            const uint32_t at = live ? kb + u : kb0, lane_at = lane * 16 + (live ? 0 : 0x80000000u);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
+            for (int j = 0; j < 2; ++j) {
 #pragma unroll
                 for (int i = 0; i < TN; ++i)
-                    o.f[i][j][e] = __builtin_amdgcn_raw_buffer_load_b128(wr, at + 2 * i * pair + j * 1024 + e * 256, 0, 0);
+                    o.f[u][i][j] = __builtin_amdgcn_raw_buffer_load_b128(wr, lane_at + j * 1024, w_at[i] + at * 2048, 0);
 #pragma unroll
                 for (int k = 0; k < TM; ++k)
-                    o.g[k][j][e] = __builtin_amdgcn_raw_buffer_load_b128(xr, at + 2 * k * pair + j * 1024 + e * 256, 0, 0);
+                    o.g[u][k][j] = __builtin_amdgcn_raw_buffer_load_b128(xr, lane_at + j * 1024, x_at[k] + at * 2048, 0);
             }
 #pragma unroll
-        for (int k = 0; k < TM; ++k) o.s[k] = live ? ld_global(s[k] + uint64_t(kb) * a.s_pitch) : 0.0f;
+            for (int k = 0; k < TM; ++k) o.s[u][k] = ld_global(s + uint64_t(at) * a.s_pitch + k * 16);
+        }
     };
-    f32x16 acc[TN][TM] = {};
+    f32x4 acc[TN][TM] = {};
     auto multiply = [&](const Operands& o, uint32_t kb) {
-        if (kb >= kb1) return;
 #pragma unroll
-        for (int i = 0; i < TN; ++i) {
-            const float by = ld_global(t[i] + kb);
+        for (int u = 0; u < U; ++u) {
+            const uint32_t at = kb + u < kb1 ? kb + u : kb0;   // past the part: operands of zeros
 #pragma unroll
-            for (int k = 0; k < TM; ++k) {
-                const f32x16 p = product32<EXACT>(o.f[i], o.g[k]);
-                const float st = o.s[k] * by;
+            for (int i = 0; i < TN; ++i) {
+                const float by = ld_uniform(t[i] + at);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[i][k][e] = __builtin_fmaf(p[e], st, acc[i][k][e]);
+                for (int k = 0; k < TM; ++k) {
+                    const f32x4 p = product16<EXACT>(o.f[u][i], o.g[u][k]);
+                    const float st = o.s[u][k] * by;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][k][e] = __builtin_fmaf(p[e], st, acc[i][k][e]);
+                }
+                if (TN * TM >= 8) __builtin_amdgcn_sched_barrier(0);   // more products in flight cost registers
             }
         }
     };
     Operands o[2];
     load(o[0], kb0);
-    for (uint32_t kb = kb0; kb < kb1; kb += 2) {
-        // the next block's loads stay ahead of this one's products
-        load(o[1], kb + 1);
+    for (uint32_t kb = kb0; kb < kb1; kb += 2 * U) {
+        // the next batch's loads stay ahead of this one's products
+        load(o[1], kb + U);
         __builtin_amdgcn_sched_barrier(0);
         multiply(o[0], kb);
         __builtin_amdgcn_sched_barrier(0);
-        load(o[0], kb + 2);
+        load(o[0], kb + 2 * U);
         __builtin_amdgcn_sched_barrier(0);
-        multiply(o[1], kb + 1);
+        multiply(o[1], kb + U);
         __builtin_amdgcn_sched_barrier(0);
     }
-    auto place = [&](int row, int unit) { return row * (BN * 4) + ((unit ^ row) & (kUnits - 1)) * 16; };
+    constexpr int kUnits = S::kUnits;
+    auto place = [&](int row, int unit) { return row * (kUnits * 16) + ((unit ^ row) & (kUnits - 1)) * 16; };
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int k = 0; k < TM; ++k)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                *reinterpret_cast<f32x4*>(smem + w * kPlane + place(k * 32 + (lane & 31), i * 8 + 2 * q + h)) =
-                    f32x4{acc[i][k][4 * q], acc[i][k][4 * q + 1], acc[i][k][4 * q + 2], acc[i][k][4 * q + 3]};
+            *reinterpret_cast<f32x4*>(smem + w * S::kPlane + place(k * 16 + (lane & 15), i * 4 + (lane >> 4))) = acc[i][k];
     __syncthreads();
-    constexpr int kOut = PAIR ? kUnits / 2 : kUnits;   // units of a row that leaves
+    constexpr int kOut = 4 * kTiles;   // units of a row that leaves
 #pragma unroll
-    for (int c = 0; c < (BM * kOut + 511) / 512; ++c) {
+    for (int c = 0; c < (16 * TM * kOut + 511) / 512; ++c) {
         const int item = c * 512 + threadIdx.x, row = item / kOut, unit = item % kOut;
-        const uint32_t m = mt * BM + row, n = nt * (kOut * 4) + unit * 4;
-        if (row >= BM || m >= a.rows || n >= a.output) continue;
+        const uint32_t m = mt * 16 * TM + row, n = c0 * 16 + unit * 4;
+        if (row >= 16 * TM || m >= a.rows || n >= a.output) continue;
         f32x4 sum{}, up{};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            sum += *reinterpret_cast<const f32x4*>(smem + j * kPlane + place(row, unit));
-            if (PAIR) up += *reinterpret_cast<const f32x4*>(smem + j * kPlane + place(row, unit + kOut));
+            sum += *reinterpret_cast<const f32x4*>(smem + j * S::kPlane + place(row, unit));
+            if (PAIR) up += *reinterpret_cast<const f32x4*>(smem + j * S::kPlane + place(row, unit + kOut));
         }
         if constexpr (PAIR) emit(a, m, n, gated4(a, n, sum, up), false);
         else emit(a, m, n, with_bias(a, n, sum), true);
@@ -319,6 +275,25 @@ hipError_t launch_core(F kernel, uint32_t tiles, uint32_t threads, size_t lds, c
     return hipGetLastError();
 }
 
+using Split16x16 = SplitShape<1, 1, 3, 4>;
+using Split16x32 = SplitShape<1, 2, 1, 4>;
+using Split32x16 = SplitShape<2, 1, 2, 4>;
+using Split32x32 = SplitShape<2, 2, 1, 4>;
+using Split32x64 = SplitShape<2, 4, 1, 2>;
+using Split64x64 = SplitShape<4, 4, 1, 2>;
+// Rows of weights x rows.  Two waves along the rows where the widening counts: a wave of 64 x 64 widens
+// less for its products than one of 128 x 32, which loads no weights that another loads too.
+template <bool EXACT>
+using Wide128x128 = WideShape<EXACT ? 4 : 8, EXACT ? 4 : 2, EXACT ? 2 : 1, EXACT ? 2 : 4, EXACT ? 1 : 2, EXACT>;
+template <bool EXACT>
+using Wide256x128 = WideShape<EXACT ? 4 : 8, EXACT ? 4 : 2, EXACT ? 2 : 1, EXACT ? 4 : 8, EXACT ? 1 : 2, EXACT>;
+using Wide256x256 = WideShape<8, 4, 2, 4, 1, false>;
+
+template <class S, bool PAIR, bool ROUNDED>
+hipError_t launch_wide(const Fp8Args& a, hipStream_t stream) {
+    return launch_core(fp8_wide_kernel<S, PAIR, ROUNDED>, a.n_tiles * a.m_tiles, S::kThreads, S::kLds, a, stream);
+}
+
 template <bool PAIR, bool EXACT>
 hipError_t launch_cores(const Fp8Plan& plan, const Fp8Layer& w, const Fp8Call& call, Fp8Args& a, hipStream_t stream) {
     if (plan.core == kFp8Decode) {
@@ -339,27 +314,35 @@ hipError_t launch_cores(const Fp8Plan& plan, const Fp8Layer& w, const Fp8Call& c
     const hipError_t e = launch_fp8_rows(call.x, call.rows, w.input, call.x_scales, blocks, scales, stream);
     if (e != hipSuccess) return e;
     const uint32_t spread = (plan.n_tiles + 7) / 8 * 8 * plan.m_tiles;
+    auto split = [&](auto shape) {
+        using S = decltype(shape);
+        if constexpr (PAIR && S::TN % 2) return hipErrorInvalidValue;
+        else return launch_core(fp8_split_kernel<S, PAIR, EXACT>, spread, 512, S::kLds, a, stream);
+    };
     switch (plan.core) {
-        case kFp8Rows16: {
-            const uint32_t groups = (w.output + 15) / 16;
-            if (a.k_blocks <= 32) return launch_core(fp8_rows16_kernel<4, PAIR>, groups, 512, 0, a, stream);
-            return launch_core(fp8_rows16_kernel<5, PAIR>, groups, 512, 0, a, stream);
-        }
-        case kFp8Direct32x32:
-            if constexpr (!PAIR) return launch_core(fp8_direct_kernel<1, 1, false, EXACT>, spread, 512, 8 * 4096, a, stream);
+        case kFp8Split16x16: return split(Split16x16{});
+        case kFp8Split16x32: return split(Split16x32{});
+        case kFp8Split32x16: return split(Split32x16{});
+        case kFp8Split32x32: return split(Split32x32{});
+        case kFp8Split32x64: return split(Split32x64{});
+        case kFp8Split64x64: return split(Split64x64{});
+        case kFp8Wide128x128: return launch_wide<Wide128x128<EXACT>, PAIR, false>(a, stream);
+        case kFp8Wide256x128:
+            if constexpr (PAIR && EXACT) {
+                if (a.y_type == kE4M3) return launch_wide<Wide256x128<true>, true, true>(a, stream);
+            }
+            return launch_wide<Wide256x128<EXACT>, PAIR, false>(a, stream);
+        case kFp8Wide256x256:
+            if constexpr (!EXACT) return launch_wide<Wide256x256, PAIR, false>(a, stream);
             return hipErrorInvalidValue;
-        case kFp8Direct32x64:
-            if constexpr (!PAIR) return launch_core(fp8_direct_kernel<1, 2, false, EXACT>, spread, 512, 8 * 8192, a, stream);
-            return hipErrorInvalidValue;
-        case kFp8Direct64x32: return launch_core(fp8_direct_kernel<2, 1, PAIR, EXACT>, spread, 512, 8 * 8192, a, stream);
-        case kFp8Direct64x64: return launch_core(fp8_direct_kernel<2, 2, PAIR, EXACT>, spread, 512, 8 * 16384, a, stream);
         default: return hipErrorInvalidValue;
     }
 }
 
 hipError_t launch_pass(const Fp8Layer& w, const Fp8Call& call, hipStream_t stream) {
-    const bool rounded = call.y.type == kE4M3;
-    const Fp8Plan plan = fp8_plan(call.rows, w.input, w.output, w.pair, rounded);
+    // e4m3 outputs come with F32 scales, which want F32's precision
+    const bool rounded = call.y.type == kE4M3, exact = call.y.type == kF32 || rounded;
+    const Fp8Plan plan = fp8_plan(call.rows, w.input, w.output, w.pair, exact, rounded);
     Fp8Args a{};
     a.w = w.blocks;
     a.t = w.scales;
@@ -379,12 +362,11 @@ hipError_t launch_pass(const Fp8Layer& w, const Fp8Call& call, hipStream_t strea
     a.y_type = call.y.type;
     a.y_scales = call.y_scales;
     float* hidden = nullptr;
-    if (rounded) {
+    if (plan.hidden) {
         a.y = hidden = reinterpret_cast<float*>(static_cast<char*>(call.workspace) + plan.hidden_at);
         a.y_stride = w.output;
         a.y_type = kF32;
     }
-    const bool exact = call.y.type == kF32;
     const hipError_t e = w.pair ? exact ? launch_cores<true, true>(plan, w, call, a, stream)
                                         : launch_cores<true, false>(plan, w, call, a, stream)
                                 : exact ? launch_cores<false, true>(plan, w, call, a, stream)
@@ -397,16 +379,26 @@ hipError_t launch_pass(const Fp8Layer& w, const Fp8Call& call, hipStream_t strea
 }  // namespace
 
 hipError_t fp8_allow_lds() {
-    const std::pair<void (*)(Fp8Args), size_t> large[] = {{fp8_direct_kernel<2, 2, false, false>, 8 * 16384},
-                                                          {fp8_direct_kernel<2, 2, false, true>, 8 * 16384},
-                                                          {fp8_direct_kernel<2, 2, true, false>, 8 * 16384},
-                                                          {fp8_direct_kernel<2, 2, true, true>, 8 * 16384}};
-    for (const auto& [kernel, lds] : large) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
-        if (e != hipSuccess) return e;
-    }
-    return hipSuccess;
+    hipError_t e = hipSuccess;
+    auto allow = [&](auto kernel, size_t lds) {
+        if (e == hipSuccess)
+            e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                    int(lds));
+    };
+    auto allow_cores = [&](auto pair) {
+        constexpr bool P = decltype(pair)::value;
+        allow(fp8_split_kernel<Split64x64, P, false>, Split64x64::kLds);
+        allow(fp8_split_kernel<Split64x64, P, true>, Split64x64::kLds);
+        allow(fp8_wide_kernel<Wide128x128<false>, P, false>, Wide128x128<false>::kLds);
+        allow(fp8_wide_kernel<Wide128x128<true>, P, false>, Wide128x128<true>::kLds);
+        allow(fp8_wide_kernel<Wide256x128<false>, P, false>, Wide256x128<false>::kLds);
+        allow(fp8_wide_kernel<Wide256x128<true>, P, false>, Wide256x128<true>::kLds);
+        allow(fp8_wide_kernel<Wide256x256, P, false>, Wide256x256::kLds);
+    };
+    allow_cores(std::false_type{});
+    allow_cores(std::true_type{});
+    allow(fp8_wide_kernel<Wide256x128<true>, true, true>, Wide256x128<true>::kLds);
+    return e;
 }
 
 hipError_t launch_fp8(const Fp8Layer& w, const Fp8Call& call, hipStream_t stream) {

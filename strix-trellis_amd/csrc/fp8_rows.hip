@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const T* x, uint64_t stri
         inv = r.inv;
     }
     put_block(blocks + (uint64_t(rb) * k_blocks + kb) * 2048, lane, in.rounded(0, inv), in.rounded(1, inv));
-    if (lane < 16 && m < rows) st_global(scales + uint64_t(kb) * s_pitch + fp8_scale_at(m), s);
+    if (lane < 16 && m < rows) st_global(scales + uint64_t(kb) * s_pitch + m, s);
 }
 
 // One workgroup per 128 x 128 block of weights: eight blocks of 16 channels, two to

@@ -219,9 +219,9 @@ static void fp8_contract(Env& e) {
     g.output_scales = buffer(os, rows * nbs);
     uint64_t need = 1, gated_need = 1;
     CHECK(strix_amd_fp8_linear_workspace_bytes(e.c, &c, &need) == kOk);
-    CHECK(need == stx::fp8_workspace_bytes(rows, I, N, false, false));
+    CHECK(need == stx::fp8_workspace_bytes(rows, I, N, false, false, false));
     CHECK(strix_amd_fp8_gated_workspace_bytes(e.c, &g, &gated_need) == kOk);
-    CHECK(gated_need == stx::fp8_workspace_bytes(rows, I, N, true, true));
+    CHECK(gated_need == stx::fp8_workspace_bytes(rows, I, N, true, true, true));
     CHECK(strix_amd_fp8_linear_workspace_bytes(e.c, &c, nullptr) == kArg);
     void* ws = device(gated_need > need ? gated_need : need);
     c.workspace = {ws, need};
@@ -498,13 +498,14 @@ static void reorder_contract(Env& e) {
 // Passes and tiles cover every row and channel within the kernels' limits.
 static void sizing() {
     // channels (of weights' rows) and rows of a tile, by core
-    const uint64_t shape[][2] = {{0, 0}, {16, 16}, {32, 32}, {32, 64}, {64, 32}, {64, 64}, {128, 128}, {256, 256}};
+    const uint64_t shape[][2] = {{0, 0},   {16, 16}, {16, 32},   {32, 16},   {32, 32},
+                                {32, 64}, {64, 64}, {128, 128}, {256, 128}, {256, 256}};
     for (uint64_t rows : {1ull, 2ull, 3ull, 4ull, 5ull, 8ull, 9ull, 16ull, 17ull, 32ull, 33ull, 64ull, 65ull, 255ull, 333ull, 2048ull, 65536ull})
         for (uint32_t I : {1u, 128u, 2048u, 2049u, 5120u, 8192u, 40000u, 131072u})
             for (uint32_t N : {1u, 16u, 512u, 5120u, 12288u, 129280u})
-                for (int kind = 0; kind < 4; ++kind) {
-                    const bool pair = kind & 1, rounded = kind == 3;
-                    const stx::Fp8Plan p = stx::fp8_plan(rows, I, N, pair, rounded);
+                for (int kind = 0; kind < 5; ++kind) {
+                    const bool pair = kind & 1, exact = kind >= 2, rounded = kind == 3;
+                    const stx::Fp8Plan p = stx::fp8_plan(rows, I, N, pair, exact, rounded);
                     const uint64_t kbs = stx::fp8_k_blocks(I);
                     if (p.core == stx::kFp8Decode) {
                         // rows in LDS, rounded up to a power of two, beside 8 KiB of sums a projection
@@ -517,16 +518,14 @@ static void sizing() {
                     }
                     CHECK(p.scales_at == stx::fp8_block_bytes(rows, I));
                     CHECK(p.bytes >= p.scales_at + kbs * stx::fp8_padded_rows(rows) * 4);
-                    if (p.hidden_at) CHECK(p.hidden_at % 256 == 0 && p.bytes >= p.hidden_at + rows * N * 4);
-                    if (p.core == stx::kFp8Rows16) {
-                        CHECK(rows <= 16);
-                        continue;
-                    }
+                    CHECK(!p.hidden || rounded);
+                    CHECK(p.core != stx::kFp8Wide256x256 || !exact);
+                    if (p.hidden) CHECK(p.hidden_at % 256 == 0 && p.bytes >= p.hidden_at + rows * N * 4);
                     const uint64_t weights = pair ? (uint64_t(N) + 31) / 32 * 64 : N;
                     CHECK(p.n_tiles == (weights + shape[p.core][0] - 1) / shape[p.core][0]);
                     CHECK(p.m_tiles == (rows + shape[p.core][1] - 1) / shape[p.core][1]);
-                    CHECK(!pair || shape[p.core][0] >= 64);
-                    if (stx::fp8_pass_rows(rows, N) == rows) CHECK(stx::fp8_workspace_bytes(rows, I, N, pair, rounded) == p.bytes);
+                    CHECK(!pair || shape[p.core][0] >= 32);
+                    if (stx::fp8_pass_rows(rows, N) == rows) CHECK(stx::fp8_workspace_bytes(rows, I, N, pair, exact, rounded) == p.bytes);
                 }
     for (uint64_t rows : {1ull, 9ull, 127ull, 128ull, 5000ull, 1ull << 20, 1ull << 31})
         for (uint32_t N : {1u, 128u, 4096u, 129280u, 16777216u}) {
@@ -534,18 +533,13 @@ static void sizing() {
             CHECK(pass >= 1 && pass <= rows && (pass == rows || pass % 128 == 0));
             CHECK(pass <= 65536);   // 16-row blocks in a side of a grid
             for (uint32_t I : {1u, 4096u, 131072u})
-                for (int pair = 0; pair < 2; ++pair)
+                for (int kind = 0; kind < 4; ++kind)
                     for (uint64_t part = 1; part <= pass; part = part < pass ? (part * 2 < pass ? part * 2 : pass) : pass + 1) {
-                        const stx::Fp8Plan p = stx::fp8_plan(part, I, N, pair, false);
+                        const stx::Fp8Plan p = stx::fp8_plan(part, I, N, kind & 1, kind & 2, false);
                         const uint64_t spread = uint64_t(p.n_tiles + 7) / 8 * 8 * p.m_tiles;
                         CHECK(spread * 512 < uint64_t(1) << 32);
                     }
         }
-    // scales of rows: every row of a 128 has a place of its own
-    for (uint32_t r = 0; r < 256; ++r) {
-        CHECK(stx::fp8_scale_at(r) / 128 == r / 128);
-        for (uint32_t s = 0; s < r; ++s) CHECK(stx::fp8_scale_at(s) != stx::fp8_scale_at(r));
-    }
     for (uint64_t rows : {1ull, 64ull, 512ull, 100000ull})
         for (uint32_t vocab : {1u, 8192u, 8193u, 129280u, 2147483647u}) {
             const uint64_t s = stx::logprobs_splits(rows, vocab), length = stx::logprobs_split_length(uint32_t(s), vocab);

@@ -63,7 +63,7 @@ hipError_t launch_fp8(const Fp8Layer& w, const Fp8Call& c, hipStream_t s) {
     require((c.y.type == kE4M3) == (c.y_scales != nullptr), "output scales");
     require(!c.x_scales || fake::in_live_block(c.x_scales, c.rows * kbs * 4), "input scales outside device memory");
     require(!c.y_scales || fake::in_live_block(c.y_scales, c.rows * nbs * 4), "output scales outside device memory");
-    const uint64_t need = fp8_workspace_bytes(c.rows, w.input, w.output, w.pair, c.y.type == kE4M3);
+    const uint64_t need = fp8_workspace_bytes(c.rows, w.input, w.output, w.pair, c.y.type == kE4M3 || c.y.type == kF32, c.y.type == kE4M3);
     require(!need || fake::in_live_block(c.workspace, need), "workspace too small");
     return note(w.pair ? "fp8_gated" : "fp8_linear", c.rows, s);
 }
