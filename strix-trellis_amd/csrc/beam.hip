@@ -1,9 +1,24 @@
 // Decoding with several beams: the selection of continuations and the reordering of states.
 //
-// Selection.  The first launch leaves, per row of logits and split of its
-// vocabulary, the softmax statistics and the `keep` first tokens in order
-// (launch_logprobs_parts).  The second has one workgroup per prompt: it joins the
-// beams' statistics, and merges the sorted lists of all beams and splits.
+// Selection.  Two launches: the first reads the logits once, and leaves for each row and
+// split of its vocabulary the softmax statistics and the `keep` first tokens in order; the second has
+// one workgroup per prompt, which joins its beams' statistics and picks among their
+// tokens.
+//
+// Statistics.  With m the largest logit of a wave so far, the wave's lanes hold
+//   s = sum e^(scale (x - m))
+// in FP32; the half steps of scale log2 e and of its product move a sum by 2^-24 (m - x) scale at most,
+// 7e-7 where all of a vocabulary of 2^17 is as likely.  A batch whose largest logit stays below m
+// needs no rescaling.  The splits' sums
+// are joined in FP64, in which the candidates' values are compared too.
+//
+// Tokens.  A token's place in the order of its row is one 64-bit key: the logit's bits,
+// made monotonic, over the inverted id.  The workgroup keeps a list of candidates in LDS and
+// a bound that at least `top` keys reach.  The first batch takes its bound from the
+// threads' largest logits (the k-th largest of each wave, with k * waves >= top).  Behind 1, 4,
+// 16, .. batches the list is cut to the first `top` keys, the last of which is the new bound: about
+// 1.4 `top` tokens enter between two cuts, and the waves meet only there.  A list that
+// overflowed in between is filled again from memory, with a higher bound.
 #include "beam.hpp"
 #include "logprobs_device.hpp"
 
@@ -11,8 +26,184 @@ namespace stx {
 
 namespace {
 
-constexpr int kThreads = 512, kWaves = kThreads / 64;
-constexpr uint32_t kList = 1024, kMaxBeams = 64;
+constexpr int kThreads = kScanThreads, kWaves = kThreads / 64;
+constexpr uint32_t kMaxBeams = 64;
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+struct ScanArgs {
+    const void* logits;
+    uint64_t stride;
+    const float* scores;         // rows with a score that is not finite are not read,
+    const int32_t* finished;     // nor finished ones
+    float* part;                 // [rows][splits]{m, s}
+    uint64_t* keys;              // [rows][splits][top]
+    uint32_t vocab, top, splits, split_length;
+    float c;                     // scale log2 e
+};
+
+// The k-th largest of a wave's values, -inf where there are fewer; k >= 1.
+__device__ __forceinline__ float kth_of_wave(float v, uint32_t k) {
+    float kth = -kInf;
+    for (;;) {
+        kth = wave_max(v);
+        if (--k == 0) return kth;
+        const uint64_t at = __ballot(v == kth);
+        if (at && (threadIdx.x & 63) == uint32_t(__builtin_ctzll(at))) v = -kInf;
+    }
+}
+
+template <class T, int EACH>
+__global__ __launch_bounds__(kThreads, 4) void beam_scan_kernel(ScanArgs a) {
+    using B = Batch<T, EACH>;
+    constexpr uint32_t kBatch = B::kBatch, kList = kScanList;
+    // batches on their way: a round trip to memory takes longer than a batch
+    constexpr int kAhead = sizeof(T) == 4 && EACH == 16 ? 2 : 3;
+    __shared__ __align__(16) uint64_t list[kList];
+    __shared__ float wave_bound[kWaves], wave_sums[kWaves];
+    __shared__ uint32_t list_end;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint64_t row = blockIdx.x / a.splits;
+    if (!(fabsf(ld_global(a.scores + row)) < kInf) || (a.finished && ld_global(a.finished + row))) return;
+    const uint32_t split = blockIdx.x % a.splits, v0 = split * a.split_length;
+    const uint32_t v1 = a.vocab - v0 < a.split_length ? a.vocab : v0 + a.split_length;
+    const T* x = static_cast<const T*>(a.logits) + row * a.stride;
+    B batch[kAhead + 1];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (v0 + i * kBatch < v1) batch[i].load(x, v0 + i * kBatch, v1);
+    float m = kLowest, s = 0.0f;   // m is the wave's
+    uint64_t bound = 0;            // keys below it do not enter the list
+    float reach = -kInf;           // its logit
+    uint32_t count = 0;            // keys in the list behind the last cut
+    float peak = -kInf;            // the thread's largest logit since then
+    uint32_t since = v0, cut_at = v0;   // the first batch since then, the batch behind which the next cut comes
+    if (tid == 0) list_end = 0;
+
+    auto weight = [&](float d) { return __builtin_amdgcn_exp2f(d * a.c); };
+    auto enter = [&](uint32_t b0, const float (&v)[EACH]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            if (!__any(v[e] >= reach)) continue;
+            const uint32_t id = B::id(b0, v1, e);
+            const uint64_t k = key_of(v[e], id);
+            if (v[e] >= reach && k >= bound && id != ~0u) {
+                const uint32_t slot = atomicAdd(&list_end, 1u);
+                if (slot < kList) list[slot] = k;
+            }
+        }
+    };
+    // A logit that at least `top` of the tokens since `since` reach, or -inf: the
+    // k-th largest peak of each wave of which every lane has tokens, the least
+    // of them.  Ends with a barrier.
+    auto reach_of_peaks = [&] {
+        const uint32_t tokens = v1 - since, of_wave = tokens / (64 * B::kGroup);
+        const uint32_t waves = of_wave < 1 ? 1 : of_wave < kWaves ? of_wave : kWaves;
+        const float kth = kth_of_wave(peak, (a.top + waves - 1) / waves);
+        if (lane == 0) wave_bound[w] = uint32_t(w) < waves ? kth : kInf;
+        __syncthreads();
+        float least = wave_bound[0];
+#pragma unroll
+        for (int i = 1; i < kWaves; ++i) least = fminf(least, wave_bound[i]);
+        __syncthreads();
+        return least;
+    };
+
+    for (uint32_t b0 = v0; b0 < v1; b0 += kBatch) {
+        if (v1 - b0 > kAhead * kBatch) batch[kAhead].load(x, b0 + kAhead * kBatch, v1);
+        float v[EACH];
+        batch[0].values(b0, v1, v);
+
+        // ---- statistics ----
+        float most = v[0];   // NaN if one is among them
+#pragma unroll
+        for (int e = 1; e < EACH; ++e) most = __builtin_elementwise_maximum(most, v[e]);
+        const float wave_most = wave_max(most);
+        if (wave_most > m) {   // the wave as one
+            s *= weight(m - wave_most);
+            m = wave_most;
+        }
+        float e2[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) e2[e] = weight(v[e] - m);
+#pragma unroll
+        for (int by = EACH / 2; by; by /= 2)   // pairwise
+#pragma unroll
+            for (int e = 0; e < by; ++e) e2[e] += e2[e + by];
+        s += e2[0];
+
+        // ---- tokens ----
+        peak = fmaxf(peak, most);
+        if (b0 == v0) {
+            reach = reach_of_peaks();
+            bound = uint64_t(key_of(reach, 0) >> 32) << 32;   // every id of that logit
+        }
+        if (__any(most >= reach)) enter(b0, v);
+        const bool last = v1 - b0 <= kBatch;
+        if (b0 == cut_at || last) {
+            __syncthreads();
+            while (list_end > kList) {
+                // More tokens than the list holds.  The peaks or, with many
+                // equal logits, the keys that got in give a higher bound; the
+                // batches since the last cut enter again behind its keys.  By
+                // the list's own bound at least kList - 2 top keys fewer do
+                // each time.
+                const uint64_t kept = uint32_t(tid) < count ? list[tid] : 0;
+                const float higher = reach_of_peaks();
+                cut(list, kList, a.top);
+                const uint64_t of_list = list[a.top - 1], of_peaks = uint64_t(key_of(higher, 0) >> 32) << 32;
+                bound = of_list > of_peaks ? of_list : of_peaks;
+                reach = value_of(bound);
+                __syncthreads();
+                if (uint32_t(tid) < count) list[tid] = kept;
+                if (tid == 0) list_end = count;
+                __syncthreads();
+                for (uint32_t b = since; b <= b0; b += kBatch) {
+                    B again;
+                    again.load(x, b, v1);
+                    float u[EACH];
+                    again.values(b, v1, u);
+                    enter(b, u);
+                }
+                __syncthreads();
+            }
+            count = cut(list, list_end, a.top);
+            if (!last) {
+                if (count == a.top) {
+                    bound = list[a.top - 1];
+                    reach = value_of(bound);
+                }
+                if (tid == 0) list_end = count;
+                since = b0 + kBatch;
+                cut_at += 3 * (cut_at - v0 + kBatch);   // behind 1, 4, 16, .. batches
+                peak = -kInf;
+                __syncthreads();
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) batch[i] = batch[i + 1];
+    }
+    // the waves' statistics as one (their peaks' place is free behind the last cut)
+    const uint64_t p = row * a.splits + split;
+    s = wave_sum(s);
+    if (lane == 0) {
+        wave_bound[w] = m;
+        wave_sums[w] = s;
+    }
+    __syncthreads();
+    if (tid < kWaves) {
+        const float of = wave_bound[tid];
+        float most = wave_bound[0];
+#pragma unroll
+        for (int i = 1; i < kWaves; ++i) most = fmaxf(most, wave_bound[i]);
+        float sum = wave_sums[tid] * weight(of - most);
+        sum += __shfl_xor(sum, 1);
+        sum += __shfl_xor(sum, 2);
+        sum += __shfl_xor(sum, 4);
+        if (tid == 0) st_global(reinterpret_cast<f32x2*>(a.part) + p, f32x2{most, sum});
+    }
+    // only the last split can be shorter than `top`: its keys end the row's
+    if (uint32_t(tid) < count) st_global(a.keys + p * a.top + tid, list[tid]);
+}
 
 struct Candidate {
     double c;
@@ -22,49 +213,68 @@ __device__ __forceinline__ bool ahead_of(const Candidate& a, const Candidate& b)
     return a.c > b.c || (a.c == b.c && a.id < b.id);
 }
 
-struct SelectArgs {
+struct JoinArgs {
     const float* scores;
     const int32_t* finished;
-    const float* part;           // [rows][splits][8]
-    const uint64_t* keys;        // [rows][splits][top]
+    const float* part;
+    const uint64_t* keys;
     float* next_scores;
     int32_t *parents, *tokens;
     uint32_t beams, keep, top, splits, last;   // last: tokens of a row's last split
     int32_t pad;
-    float c;
-    double scale, slope;         // slope: (scale log2 e - c) / c ln 2
+    double scale;
 };
 
-__global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectArgs a) {
+// The beams' lists of keys, first keys first, are taken 1024 at a time (nearly always all of them at
+// once); what reaches a bound that `keep` of them reach enters a list in LDS, whose first `keep` are
+// found by counting who is ahead of whom.  The lists are sorted, so behind a round of which none
+// enters there is nothing.
+__global__ __launch_bounds__(kThreads) void beam_join_kernel(JoinArgs a) {
+    constexpr uint32_t kRound = 2 * kThreads, kList = kRound + 2 * kMaxBeams;   // + kept ones and pad tokens
     __shared__ Candidate list[kList];
-    __shared__ double beam_at[kMaxBeams];    // a candidate's value is beam_at + scale * (logit - beam_m)
+    __shared__ double beam_at[kMaxBeams];       // a candidate's value is beam_at + scale * (logit - beam_m)
     __shared__ float beam_m[kMaxBeams];
     __shared__ uint32_t beam_kind[kMaxBeams];   // 0 offers nothing, 1 its tokens, 2 the pad token
+    __shared__ float wave_bound[kWaves];
     __shared__ uint32_t list_end;
     const uint32_t tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint64_t row0 = uint64_t(blockIdx.x) * a.beams;
+    const uint32_t lists = a.beams * a.splits, all = lists * a.top;
+    // A round's items by depth in their lists, dealt out to the waves in turn, another one first each time:
+    // the waves' bounds are as high as their first keys are evenly spread.
+    auto key_at = [&](uint32_t i) -> uint64_t {
+        const uint32_t d = i / lists, l = i - d * lists, split = l % a.splits;
+        const uint32_t length = split + 1 < a.splits || a.last > a.top ? a.top : a.last;
+        return i < all && d < length ? ld_global(a.keys + (row0 * a.splits + l) * a.top + d) : 0;
+    };
+    // of rows that were not read they hold anything, and are not used
+    uint64_t key[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) key[j] = key_at(j * kThreads + lane * kWaves + ((w + lane) % kWaves));
     if (tid == 0) list_end = 0;
     for (uint32_t b = w; b < a.beams; b += kWaves) {
+        const f32x2* from = reinterpret_cast<const f32x2*>(a.part) + (row0 + b) * a.splits;
+        const f32x2 none = {kLowest, 0.0f}, first = lane < a.splits ? ld_global(from + lane) : none;
         const float score = ld_global(a.scores + row0 + b);
         const bool over = a.finished && ld_global(a.finished + row0 + b) != 0;
         uint32_t kind = 0;
         double at = score;
-        float m = 0.0f;
+        float m = first[0];
         if (fabsf(score) < kInf) {
             kind = 2;
             if (!over) {
-                Stats t = kNothing;
-                for (uint32_t i = lane; i < a.splits; i += 64) {
-                    const f32x4 o = ld_global(reinterpret_cast<const f32x4*>(a.part + ((row0 + b) * a.splits + i) * 8));
-                    join(t, {o[0], o[1], o[2], o[3]}, a.c);
-                }
-                t = join_lanes(t, a.c);
-                kind = t.n > 0.0f && t.m < kInf && t.s == t.s ? 1 : 0;
-                // The statistics were taken at c, scale log2 e rounded to FP32: the first
-                // order of the log sum in the difference, whose square is below 1e-14.
-                const double sum = double(t.n) + double(t.s);
-                at = double(score) - (log(sum) + a.slope * double(t.h) / sum);
-                m = t.m;
+                for (uint32_t i = lane + 64; i < a.splits; i += 64) m = fmaxf(m, ld_global(from + i)[0]);
+                m = wave_max(m);
+                // a split that had no logit above -inf has a sum of 0
+                auto joined = [&](f32x2 o) {
+                    return o[1] == 0.0f ? 0.0 : double(o[1]) * exp(a.scale * (double(o[0]) - double(m)));
+                };
+                double sum = joined(first);
+                for (uint32_t i = lane + 64; i < a.splits; i += 64) sum += joined(ld_global(from + i));
+#pragma unroll
+                for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+                kind = sum > 0.0 && m < kInf ? 1 : 0;   // neither where it is NaN
+                at = double(score) - log(sum);
             }
         }
         if (lane == 0) {
@@ -75,45 +285,71 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectArgs a) {
     }
     __syncthreads();
 
-    // The lists, first keys first: rounds of about 128 keys that enter if they beat
-    // the last of the best so far.  The lists are sorted, so a round of which
-    // none enters is the last.
-    const uint32_t lists = a.beams * a.splits, depth = lists >= 128 ? 1 : 128 / lists;
     uint32_t count = 0;
-    Candidate bound{-double(kInf), ~uint64_t(0)};
-    for (uint32_t d0 = 0; d0 < a.top; d0 += depth) {
-        auto enter = [&](const Candidate& k) {
-            if (k.c == -double(kInf) || (count == a.keep && !ahead_of(k, bound))) return;
-            list[atomicAdd(&list_end, 1u)] = k;   // 64 kept, 64 finished and 512 others at most
-        };
-        if (d0 == 0 && tid < a.beams && beam_kind[tid] == 2)
-            enter({beam_at[tid], uint64_t(tid) << 32 | uint32_t(a.pad)});
-        for (uint32_t i = tid; i < lists * depth; i += kThreads) {
-            const uint32_t l = i % lists, d = d0 + i / lists, b = l / a.splits, split = l % a.splits;
-            const uint32_t length = split + 1 < a.splits || a.last > a.top ? a.top : a.last;
-            if (d >= length || beam_kind[b] != 1) continue;
-            const uint64_t key = ld_global(a.keys + ((row0 + b) * a.splits + split) * a.top + d);
-            const double x = value_of(key);
-            enter({beam_at[b] + a.scale * (x - double(beam_m[b])), uint64_t(b) << 32 | id_of(key)});
+    Candidate bound{-double(kInf), ~uint64_t(0)};   // the last of the kept ones
+    for (uint32_t i0 = 0; i0 < all; i0 += kRound) {
+        Candidate mine[3];
+        float most = -kInf;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t i = i0 + j * kThreads + lane * kWaves + ((w + lane) % kWaves), l = i % lists, b = l / a.splits;
+            if (i0) key[j] = key_at(i);
+            mine[j].c = -double(kInf);
+            if (key[j] && beam_kind[b] == 1)
+                mine[j] = {beam_at[b] + a.scale * (double(value_of(key[j])) - double(beam_m[b])),
+                           uint64_t(b) << 32 | id_of(key[j])};
+            most = fmaxf(most, float(mine[j].c));
+        }
+        mine[2].c = -double(kInf);
+        if (i0 == 0 && tid < a.beams && beam_kind[tid] == 2) mine[2] = {beam_at[tid], uint64_t(tid) << 32 | uint32_t(a.pad)};
+        // the least of the waves' k-th largest, with k * waves >= keep (FP32 keeps the order)
+        float reach = -kInf;
+        if (i0 == 0) {
+            const float kth = kth_of_wave(most, (a.keep + kWaves - 1) / kWaves);
+            if (lane == 0) wave_bound[w] = kth;
+            __syncthreads();
+            reach = wave_bound[0];
+#pragma unroll
+            for (int j = 1; j < kWaves; ++j) reach = fminf(reach, wave_bound[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+            const Candidate& k = mine[j];
+            if (k.c == -double(kInf) || float(k.c) < reach || (count == a.keep && !ahead_of(k, bound))) continue;
+            list[atomicAdd(&list_end, 1u)] = k;
         }
         __syncthreads();
         const uint32_t n = list_end;
-        if (n == count && d0) break;
-        Candidate mine[2];
-        uint32_t rank[2] = {0, 0};
+        if (n == count && i0) break;
+        // who is ahead of whom: eight threads to a candidate where that takes them all at once
+        if (n <= kThreads / 8) {
+            const uint32_t i = tid >> 3, part = tid & 7;
+            const Candidate mine = list[i];
+            uint32_t ahead = 0;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) mine[j] = tid + j * kThreads < n ? list[tid + j * kThreads] : Candidate{0.0, 0};
-        if (uint32_t(__builtin_amdgcn_readfirstlane(tid)) < n) {   // the wave holds candidates
+            for (int j = 0; j < 8; ++j) ahead += part + 8 * j < n && ahead_of(list[part + 8 * j], mine);
+            ahead += __builtin_amdgcn_update_dpp(0, ahead, 0xB1, 0xf, 0xf, true);    // quad_perm 1,0,3,2
+            ahead += __builtin_amdgcn_update_dpp(0, ahead, 0x4E, 0xf, 0xf, true);    // quad_perm 2,3,0,1
+            ahead += __builtin_amdgcn_update_dpp(0, ahead, 0x141, 0xf, 0xf, true);   // row_half_mirror
+            __syncthreads();
+            if (part == 0 && i < n && ahead < a.keep) list[ahead] = mine;
+        } else {
+            constexpr int kEach = (kList + kThreads - 1) / kThreads;
+            Candidate k[kEach];
+            uint32_t ahead[kEach] = {};
+#pragma unroll
+            for (int j = 0; j < kEach; ++j)
+                if (tid + j * kThreads < n) k[j] = list[tid + j * kThreads];
             for (uint32_t i = 0; i < n; ++i) {
-                const Candidate k = list[i];
+                const Candidate o = list[i];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) rank[j] += ahead_of(k, mine[j]);
+                for (int j = 0; j < kEach; ++j) ahead[j] += ahead_of(o, k[j]);
             }
-        }
-        __syncthreads();
+            __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-            if (tid + j * kThreads < n && rank[j] < a.keep) list[rank[j]] = mine[j];
+            for (int j = 0; j < kEach; ++j)
+                if (tid + j * kThreads < n && ahead[j] < a.keep) list[ahead[j]] = k[j];
+        }
         count = n < a.keep ? n : a.keep;
         if (tid == 0) list_end = count;
         __syncthreads();
@@ -126,6 +362,15 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectArgs a) {
         st_global(a.parents + to, int32_t(k.id >> 32));
         st_global(a.tokens + to, int32_t(uint32_t(k.id)));
     }
+}
+
+template <class T>
+hipError_t scan(const ScanArgs& a, const BeamSplits& splits, uint64_t rows, hipStream_t stream) {
+    constexpr int kSmall = 16 / sizeof(T);
+    const dim3 grid(a.splits * uint32_t(rows));
+    if (splits.each == 16) hipLaunchKernelGGL((beam_scan_kernel<T, 16>), grid, dim3(kThreads), 0, stream, a);
+    else hipLaunchKernelGGL((beam_scan_kernel<T, kSmall>), grid, dim3(kThreads), 0, stream, a);
+    return hipGetLastError();
 }
 
 // ---- reordering ----
@@ -248,41 +493,69 @@ hipError_t reorder(const BeamReorderCall& call, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_beam_select(const BeamSelectCall& call, hipStream_t stream) {
-    SelectArgs a{};
+    const BeamSplits splits = beam_splits(call.rows, call.vocab, call.logits.type);
+    const uint32_t top = call.keep < call.vocab ? call.keep : call.vocab;
+    auto* part = static_cast<float*>(call.workspace);
+    auto* keys = reinterpret_cast<uint64_t*>(part + call.rows * splits.splits * 2);
+    ScanArgs a{};
+    a.logits = call.logits.data;
+    a.stride = call.logits.stride;
     a.scores = call.scores;
     a.finished = call.finished;
-    a.next_scores = call.next_scores;
-    a.parents = call.parents;
-    a.tokens = call.tokens;
-    a.beams = call.beams;
-    a.keep = call.keep;
-    a.top = call.keep < call.vocab ? call.keep : call.vocab;
-    a.splits = logprobs_splits(call.rows, call.vocab);
-    a.last = call.vocab - (a.splits - 1) * logprobs_split_length(a.splits, call.vocab);
-    a.pad = call.pad;
-    a.c = logprobs_exponent(call.scale);
-    const double c = double(call.scale) * 1.4426950408889634074;
-    a.scale = call.scale;
-    a.slope = (c - double(a.c)) / double(a.c) * 0.69314718055994530942;
-    a.part = static_cast<const float*>(call.workspace);
-    a.keys = reinterpret_cast<const uint64_t*>(a.part + call.rows * a.splits * 8);
-    const hipError_t e = launch_logprobs_parts(call.logits, call.rows, call.vocab, a.top, call.scale, call.scores,
-                                               call.finished, call.workspace, stream);
-    if (e != hipSuccess) return e;
+    a.part = part;
+    a.keys = keys;
+    a.vocab = call.vocab;
+    a.top = top;
+    a.splits = splits.splits;
+    a.split_length = splits.length;
+    a.c = float(double(call.scale) * 1.4426950408889634074);
+    JoinArgs j{};
+    j.scores = call.scores;
+    j.finished = call.finished;
+    j.part = part;
+    j.keys = keys;
+    j.next_scores = call.next_scores;
+    j.parents = call.parents;
+    j.tokens = call.tokens;
+    j.beams = call.beams;
+    j.keep = call.keep;
+    j.top = top;
+    j.splits = splits.splits;
+    j.last = call.vocab - (splits.splits - 1) * splits.length;
+    j.pad = call.pad;
+    j.scale = call.scale;
+    // a launch holds fewer than 2^32 threads (rows in such numbers take one split)
+    constexpr uint64_t kRows = 1u << 20;
+    for (uint64_t left = call.rows; left;) {
+        const uint64_t n = left < kRows ? left : kRows;
+        hipError_t e = hipErrorInvalidValue;
+        switch (call.logits.type) {
+            case kF32: e = scan<float>(a, splits, n, stream); break;
+            case kF16: e = scan<_Float16>(a, splits, n, stream); break;
+            case kBF16: e = scan<__bf16>(a, splits, n, stream); break;
+        }
+        if (e != hipSuccess) return e;
+        left -= n;
+        a.logits = static_cast<const char*>(a.logits) + n * a.stride * (call.logits.type == kF32 ? 4 : 2);
+        a.scores += n;
+        if (a.finished) a.finished += n;
+        a.part += n * splits.splits * 2;
+        a.keys += n * splits.splits * top;
+    }
     const uint64_t prompts = call.rows / call.beams;
-    constexpr uint64_t kPrompts = 1u << 22;   // a launch holds fewer than 2^32 threads
+    constexpr uint64_t kPrompts = 1u << 22;
     for (uint64_t p = 0; p < prompts; p += kPrompts) {
         const uint64_t n = prompts - p < kPrompts ? prompts - p : kPrompts;
-        hipLaunchKernelGGL(beam_join_kernel, dim3(uint32_t(n)), dim3(kThreads), 0, stream, a);
-        const hipError_t joined = hipGetLastError();
-        if (joined != hipSuccess) return joined;
-        a.scores += n * a.beams;
-        if (a.finished) a.finished += n * a.beams;
-        a.part += n * a.beams * a.splits * 8;
-        a.keys += n * a.beams * a.splits * a.top;
-        a.next_scores += n * a.keep;
-        a.parents += n * a.keep;
-        a.tokens += n * a.keep;
+        hipLaunchKernelGGL(beam_join_kernel, dim3(uint32_t(n)), dim3(kThreads), 0, stream, j);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        j.scores += n * j.beams;
+        if (j.finished) j.finished += n * j.beams;
+        j.part += n * j.beams * splits.splits * 2;
+        j.keys += n * j.beams * splits.splits * top;
+        j.next_scores += n * j.keep;
+        j.parents += n * j.keep;
+        j.tokens += n * j.keep;
     }
     return hipSuccess;
 }

@@ -17,7 +17,13 @@ struct BeamSelectCall {
     float scale = 1.0f;
     void* workspace = nullptr;
 };
-uint64_t beam_select_workspace_bytes(uint64_t rows, uint32_t vocab, uint32_t keep);
+// How a row of logits is read: in batches of 512 threads x `each` logits, and in splits of whole
+// batches, a workgroup each.
+struct BeamSplits {
+    uint32_t each = 16, splits = 1, length = 0;
+};
+BeamSplits beam_splits(uint64_t rows, uint32_t vocab, uint32_t type);
+uint64_t beam_select_workspace_bytes(uint64_t rows, uint32_t vocab, uint32_t type, uint32_t keep);
 hipError_t launch_beam_select(const BeamSelectCall& call, hipStream_t stream);
 
 struct BeamReorderCall {

@@ -24,7 +24,7 @@ strix_status describe_select(strix_context c, const strix_amd_beam_select_desc* 
                d->keep <= STRIX_AMD_MAX_TOP && rows % d->beams == 0,
            STRIX_ERROR_UNSUPPORTED_FORMAT);
     if (!r.held()) return r.status();
-    need = rows ? stx::beam_select_workspace_bytes(rows, uint32_t(x.width), d->keep) : 0;
+    need = rows ? stx::beam_select_workspace_bytes(rows, uint32_t(x.width), x.at.type, d->keep) : 0;
     if (!place) return STRIX_SUCCESS;
     const uint64_t places = rows / d->beams * d->keep;
     Span scores, finished, next_scores, parents, tokens, workspace;

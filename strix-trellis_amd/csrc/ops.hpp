@@ -106,15 +106,5 @@ constexpr uint32_t kLogprobsBatch = 8192;
 uint32_t logprobs_splits(uint64_t rows, uint32_t vocab);
 uint64_t logprobs_workspace_bytes(uint64_t rows, uint32_t vocab, uint32_t top);
 hipError_t launch_token_logprobs(const LogprobsCall& call, hipStream_t stream);
-// scale log2 e as the kernels hold it, and the logits of a split.
-inline float logprobs_exponent(float scale) { return float(double(scale) * 1.4426950408889634074); }
-constexpr uint32_t logprobs_split_length(uint32_t splits, uint32_t vocab) {
-    return uint32_t(((uint64_t(vocab) + kLogprobsBatch - 1) / kLogprobsBatch + splits - 1) / splits) * kLogprobsBatch;
-}
-// Per row and split its statistics ([rows][splits][8] words: largest logit, count of it,
-// sums) and its `top` first keys ([rows][splits][top], fewer of a shorter last split), of the
-// rows with a finite score that are not finished; the others' are left as they are.
-hipError_t launch_logprobs_parts(const OpRows& logits, uint64_t rows, uint32_t vocab, uint32_t top, float scale,
-                                 const float* scores, const int32_t* finished, void* workspace, hipStream_t stream);
 
 }  // namespace stx

@@ -44,17 +44,43 @@ namespace stx {
 
 namespace {
 
-constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kThreads = kScanThreads, kWaves = kThreads / 64;
 constexpr int kEach = 16;                               // logits per thread and batch
 constexpr uint32_t kBatch = kThreads * kEach;
 static_assert(kBatch == kLogprobsBatch);
-constexpr uint32_t kList = 1024;                        // candidate capacity
+constexpr uint32_t kList = kScanList;                   // candidate capacity
 constexpr float kLn2 = 0.69314718055994530942f;
 
 // The next float above x (x not NaN or +inf).
 __device__ __forceinline__ float above(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
     return __builtin_bit_cast(float, b & 0x80000000u ? b - 1 : b + 1);
+}
+
+struct Stats {
+    float m, n, s, h;
+};
+constexpr Stats kNothing = {kLowest, 0.0f, 0.0f, 0.0f};
+
+// Distances past 2^24 have no weight at any admitted scale (2^24 times 2^-16
+// log2 e is over 300); kept finite, a weight of 0 times one is 0.
+__device__ __forceinline__ float power(float d, float c) { return fmaxf(d, -0x1p24f) * c; }
+
+// Statistics p against the larger maximum m.
+__device__ __forceinline__ Stats against(const Stats& p, float m, float c) {
+    const float d = power(p.m - m, c), f = __builtin_amdgcn_exp2f(d), t = p.n + p.s;
+    return p.m == m ? p : Stats{m, 0.0f, f * t, f * __builtin_fmaf(t, d, p.h)};
+}
+__device__ __forceinline__ void join(Stats& a, const Stats& b, float c) {
+    const float m = fmaxf(a.m, b.m);
+    const Stats x = against(a, m, c), y = against(b, m, c);
+    a = {m, x.n + y.n, x.s + y.s, x.h + y.h};
+}
+// Joins the lanes' statistics; every lane gets the result.
+__device__ __forceinline__ Stats join_lanes(const Stats& mine, float c) {
+    const float m = wave_max(mine.m);
+    const Stats x = against(mine, m, c);
+    return {m, wave_sum(x.n), wave_sum(x.s), wave_sum(x.h)};
 }
 
 // What the statistics of a whole row say; invalid rows give NaN.
@@ -85,63 +111,7 @@ struct Args {
     // ([rows][splits][8] words), then the keys ([rows][splits][top]).
     float* part;
     uint64_t* part_keys;
-    // PARTS: rows that are read (a finite score, not finished)
-    const float* scores;
-    const int32_t* finished;
 };
-
-// Sorts the first `top` of list[0..count) to its front (largest first) and
-// returns how many there are.  All threads call it; ends with a barrier.
-// Ranks by counting (every key is distinct).  Up to 64 keys, the usual cut of a
-// few tokens, are spread over all threads and take one LDS round trip (512 x
-// 129280 BF16, 20 tokens, 42.0 -> 40.1 us; 33 x 100277, 5 tokens, 12.7 -> 11.9: tokens and
-// entropy of the same normal logits each time, from the last-level cache); more go a key
-// or two to a thread, eight of the list in flight per step, and keys past the count are
-// 0, which is ahead of none.
-__device__ __forceinline__ uint32_t cut(uint64_t* list, uint32_t count, uint32_t top) {
-    typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
-    if (count <= kThreads / 8) {   // eight threads to a key, eight keys each
-        const uint32_t i = threadIdx.x >> 3, part = threadIdx.x & 7;
-        __syncthreads();
-        const uint64_t mine = list[i];
-        uint64_t k[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) k[j] = list[part + 8 * j];
-        uint32_t ahead = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ahead += part + 8 * j < count && k[j] > mine;
-        ahead += __builtin_amdgcn_update_dpp(0, ahead, 0xB1, 0xf, 0xf, true);    // quad_perm 1,0,3,2
-        ahead += __builtin_amdgcn_update_dpp(0, ahead, 0x4E, 0xf, 0xf, true);    // quad_perm 2,3,0,1
-        ahead += __builtin_amdgcn_update_dpp(0, ahead, 0x141, 0xf, 0xf, true);   // row_half_mirror
-        __syncthreads();
-        if (part == 0 && i < count && ahead < top) list[ahead] = mine;
-        __syncthreads();
-        return count < top ? count : top;
-    }
-    const uint32_t i0 = threadIdx.x, i1 = threadIdx.x + kThreads, padded = (count + 7) & ~7u;
-    if (count + i0 < padded) list[count + i0] = 0;
-    __syncthreads();
-    const uint64_t k0 = i0 < count ? list[i0] : 0, k1 = i1 < count ? list[i1] : 0;
-    uint32_t a0 = 0, a1 = 0;
-    if (uint32_t(__builtin_amdgcn_readfirstlane(i0)) < count) {   // the wave holds keys
-        for (uint32_t i = 0; i < padded; i += 8) {
-            u64x2 k[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const u64x2*>(list + i + 2 * j);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) a0 += (k[j][0] > k0) + (k[j][1] > k0);
-            if (count > kThreads) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) a1 += (k[j][0] > k1) + (k[j][1] > k1);
-            }
-        }
-    }
-    __syncthreads();
-    if (i0 < count && a0 < top) list[a0] = k0;
-    if (i1 < count && a1 < top) list[a1] = k1;
-    __syncthreads();
-    return count < top ? count : top;
-}
 
 // Writes the row's results from its statistics, the tokens ahead of the given
 // one, and the sorted list of its first tokens.
@@ -166,53 +136,7 @@ __device__ __forceinline__ void finish(const Args& a, uint64_t row, const Stats&
     }
 }
 
-// A thread's logits of a batch as loaded: groups of 16 bytes, the workgroup's
-// groups side by side.
 template <class T>
-struct Batch {
-    static constexpr int kGroup = 16 / sizeof(T), kGroups = kEach / kGroup;
-    typename Packed<T, kGroup>::type raw[kGroups];
-
-    static __device__ __forceinline__ uint32_t first(int g) { return (g * kThreads + threadIdx.x) * kGroup; }
-    // A group that would reach past v1 is loaded where it ends at v1: its first
-    // logits are another group's, and drop out by `id`.
-    static __device__ __forceinline__ uint32_t place(uint32_t b0, uint32_t v1, int g) {
-        const uint32_t k = b0 + first(g);
-        return k < v1 - kGroup ? k : v1 - kGroup;
-    }
-    __device__ __forceinline__ void load(const T* x, uint32_t b0, uint32_t v1) {
-        if (b0 + kBatch <= v1) {
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) raw[g] = ld_packed<kGroup>(x + b0 + first(g));
-        } else if (v1 >= uint32_t(kGroup)) {
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) raw[g] = ld_packed<kGroup>(x + place(b0, v1, g));
-        } else {
-#pragma unroll
-            for (int i = 0; i < kGroup; ++i) raw[0][i] = uint32_t(i) < v1 ? ld_global(x + i) : T(-kInf);
-        }
-    }
-    // Token of element e, ~0 where another element is that token or there is none.
-    static __device__ __forceinline__ uint32_t id(uint32_t b0, uint32_t v1, int e) {
-        const uint32_t k = b0 + first(e / kGroup);
-        if (b0 + kBatch <= v1) return k + e % kGroup;
-        if (v1 < uint32_t(kGroup)) return k + e % kGroup < v1 ? k + e % kGroup : ~0u;
-        const uint32_t i = place(b0, v1, e / kGroup) + e % kGroup;
-        return i >= k ? i : ~0u;
-    }
-    // The logits, -inf where `id` gives none.
-    __device__ __forceinline__ void values(uint32_t b0, uint32_t v1, float (&v)[kEach]) const {
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) v[e] = float(raw[e / kGroup][e % kGroup]);
-        if (b0 + kBatch > v1) {
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) v[e] = id(b0, v1, e) != ~0u ? v[e] : -kInf;
-        }
-    }
-};
-
-// PARTS: the statistics and keys alone, of any number of splits, for another join.
-template <class T, bool PARTS>
 __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(Args a) {
     __shared__ __align__(16) uint64_t list[kList];
     __shared__ float wave_bound[kWaves];
@@ -224,10 +148,7 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(Args a) {
     const uint32_t split = blockIdx.x % a.splits, v0 = split * a.split_length;
     const uint32_t v1 = a.vocab - v0 < a.split_length ? a.vocab : v0 + a.split_length;
     const T* x = static_cast<const T*>(a.logits) + row * a.stride;
-    if constexpr (PARTS) {
-        if (!(fabsf(ld_global(a.scores + row)) < kInf) || (a.finished && ld_global(a.finished + row))) return;
-    }
-    using B = Batch<T>;
+    using B = Batch<T, kEach>;
     const uint32_t token = a.tokens ? uint32_t(ld_global(a.tokens + row)) : ~0u;   // first: its logit's address
     B batch, next, later;   // two batches ahead: a round trip to memory takes longer than a batch
     batch.load(x, v0, v1);
@@ -384,7 +305,7 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(Args a) {
     ahead = 0;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) ahead += wave_ahead[i];
-    if (!PARTS && a.splits == 1) {
+    if (a.splits == 1) {
         finish(a, row, t, token, given, ahead, list);
         return;
     }
@@ -477,55 +398,14 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(Args a) {
 
 template <class T>
 hipError_t dispatch(const Args& a, uint64_t rows, hipStream_t stream) {
-    hipLaunchKernelGGL((token_logprobs_kernel<T, false>), dim3(a.splits * uint32_t(rows)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(token_logprobs_kernel<T>, dim3(a.splits * uint32_t(rows)), dim3(kThreads), 0, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
     hipLaunchKernelGGL(token_logprobs_join_kernel<T>, dim3(uint32_t(rows)), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
 
-template <class T>
-hipError_t dispatch_parts(const Args& a, uint64_t rows, hipStream_t stream) {
-    hipLaunchKernelGGL((token_logprobs_kernel<T, true>), dim3(a.splits * uint32_t(rows)), dim3(kThreads), 0, stream, a);
-    return hipGetLastError();
-}
-
 }  // namespace
-
-hipError_t launch_logprobs_parts(const OpRows& logits, uint64_t rows, uint32_t vocab, uint32_t top, float scale,
-                                 const float* scores, const int32_t* finished, void* workspace, hipStream_t stream) {
-    Args a{};
-    a.logits = logits.data;
-    a.stride = logits.stride;
-    a.vocab = vocab;
-    a.top = top;
-    a.scale = scale;
-    a.c = logprobs_exponent(scale);
-    a.splits = logprobs_splits(rows, vocab);
-    a.split_length = logprobs_split_length(a.splits, vocab);
-    a.part = static_cast<float*>(workspace);
-    a.part_keys = reinterpret_cast<uint64_t*>(a.part + rows * a.splits * 8);
-    a.scores = scores;
-    a.finished = finished;
-    constexpr uint64_t kRows = 1u << 20;   // a launch holds fewer than 2^32 threads
-    for (uint64_t left = rows; left;) {
-        const uint64_t n = left < kRows ? left : kRows;
-        hipError_t e = hipErrorInvalidValue;
-        switch (logits.type) {
-            case kF32: e = dispatch_parts<float>(a, n, stream); break;
-            case kF16: e = dispatch_parts<_Float16>(a, n, stream); break;
-            case kBF16: e = dispatch_parts<__bf16>(a, n, stream); break;
-        }
-        if (e != hipSuccess) return e;
-        left -= n;
-        a.logits = static_cast<const char*>(a.logits) + n * a.stride * (logits.type == kF32 ? 4 : 2);
-        a.scores += n;
-        if (a.finished) a.finished += n;
-        a.part += n * a.splits * 8;
-        a.part_keys += n * a.splits * top;
-    }
-    return hipSuccess;
-}
 
 hipError_t launch_token_logprobs(const LogprobsCall& call, hipStream_t stream) {
     Args a{};
@@ -540,9 +420,10 @@ hipError_t launch_token_logprobs(const LogprobsCall& call, hipStream_t stream) {
     a.vocab = call.vocab;
     a.top = call.top;
     a.scale = call.scale;
-    a.c = logprobs_exponent(call.scale);
+    a.c = float(double(call.scale) * 1.4426950408889634074);
+    const uint64_t batches = (uint64_t(call.vocab) + kBatch - 1) / kBatch;
     a.splits = logprobs_splits(call.rows, call.vocab);
-    a.split_length = logprobs_split_length(a.splits, call.vocab);
+    a.split_length = uint32_t((batches + a.splits - 1) / a.splits) * kBatch;
     a.part = static_cast<float*>(call.workspace);
     a.part_keys = reinterpret_cast<uint64_t*>(a.part + call.rows * a.splits * 8);
     // a launch holds fewer than 2^32 threads (more rows than that take one split)

@@ -353,7 +353,7 @@ static void select_contract(Env& e) {
     d.scale = 1;
     uint64_t need = 0;
     CHECK(strix_amd_beam_select_workspace_bytes(e.c, &d, &need) == kOk);
-    CHECK(need == stx::beam_select_workspace_bytes(rows, vocab, keep) && need);
+    CHECK(need == stx::beam_select_workspace_bytes(rows, vocab, F32, keep) && need);
     void* ws = device(need);
     d.workspace = {ws, need};
     auto call = [&](const strix_amd_beam_select_desc& y) {
@@ -540,12 +540,16 @@ static void sizing() {
                         CHECK(spread * 512 < uint64_t(1) << 32);
                     }
         }
-    for (uint64_t rows : {1ull, 64ull, 512ull, 100000ull})
-        for (uint32_t vocab : {1u, 8192u, 8193u, 129280u, 2147483647u}) {
-            const uint64_t s = stx::logprobs_splits(rows, vocab), length = stx::logprobs_split_length(uint32_t(s), vocab);
-            CHECK((s - 1) * length < vocab && s * length >= vocab);
-            CHECK(stx::beam_select_workspace_bytes(rows, vocab, 64) >= rows * s * (32 + (vocab < 64 ? vocab : 64) * 8));
-        }
+    for (uint64_t rows : {1ull, 4ull, 64ull, 511ull, 512ull, 100000ull})
+        for (uint32_t vocab : {1u, 2048u, 8192u, 8193u, 129280u, 2147483647u})
+            for (uint32_t type : {F32, BF16}) {
+                const stx::BeamSplits s = stx::beam_splits(rows, vocab, type);
+                CHECK(s.each == 16 || s.each == (type == F32 ? 4 : 8));
+                CHECK(s.length % (512 * s.each) == 0 && (s.splits == 1 || s.splits * rows <= 512));
+                CHECK(uint64_t(s.splits - 1) * s.length < vocab && uint64_t(s.splits) * s.length >= vocab);
+                CHECK(stx::beam_select_workspace_bytes(rows, vocab, type, 64) >=
+                      rows * s.splits * (8 + (vocab < 64 ? vocab : 64) * 8));
+            }
 }
 
 int main() {

@@ -75,7 +75,7 @@ hipError_t launch_beam_select(const BeamSelectCall& c, hipStream_t s) {
     require(!c.finished || fake::in_live_block(c.finished, c.rows * 4), "flags outside device memory");
     for (const void* v : {(const void*)c.next_scores, (const void*)c.parents, (const void*)c.tokens})
         require(fake::in_live_block(v, c.rows / c.beams * c.keep * 4), "results outside device memory");
-    require(fake::in_live_block(c.workspace, beam_select_workspace_bytes(c.rows, c.vocab, c.keep)), "workspace too small");
+    require(fake::in_live_block(c.workspace, beam_select_workspace_bytes(c.rows, c.vocab, c.logits.type, c.keep)), "workspace too small");
     return note("beam_select", c.rows, s);
 }
 
