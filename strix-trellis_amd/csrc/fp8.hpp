@@ -75,7 +75,6 @@ struct Fp8Plan {
     uint64_t scales_at = 0, hidden_at = 0, bytes = 0;
     bool hidden = false;   // F32 rows in the workspace that another launch rounds to e4m3
 };
-constexpr uint32_t kFp8DecodeLds = 44 * 1024;   // rows and scales of a decode launch in LDS
 // exact: products in FP32 whole (F32 and e4m3 outputs); rounded: e4m3 output.
 uint64_t fp8_pass_rows(uint64_t rows, uint32_t output);
 Fp8Plan fp8_plan(uint64_t rows, uint32_t input, uint32_t output, bool pair, bool exact, bool rounded);

@@ -7,7 +7,6 @@
 namespace stx {
 
 typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr float kLeastScale = 0x1p-126f;
 
@@ -19,10 +18,20 @@ __device__ __forceinline__ float maximum(float a, float b) { return __builtin_el
 struct BlockScale {
     float s, inv;
 };
+// Both quotients are the rounded ones, in fewer steps than a division takes that has to
+// reach every pair of operands: q corrected once by its residual is RN32(most / 448) for every `most` of
+// which it counts; two Newton steps from a reciprocal that is off by at most a unit give
+// RN32(1 / s) (each proved by trying every mantissa).  Only an infinity needs a step of its own.
 __device__ __forceinline__ BlockScale block_scale(float most) {
+    constexpr float kBy = 1.0f / 448.0f;
     BlockScale r;
-    r.s = maximum(most / 448.0f, kLeastScale);
-    r.inv = 1.0f / r.s;
+    const bool infinite = most == __builtin_inff();
+    const float q = most * kBy, s = maximum(__builtin_fmaf(__builtin_fmaf(-448.0f, q, most), kBy, q), kLeastScale);
+    float y = __builtin_amdgcn_rcpf(s);
+    y = __builtin_fmaf(__builtin_fmaf(-s, y, 1.0f), y, y);
+    y = __builtin_fmaf(__builtin_fmaf(-s, y, 1.0f), y, y);
+    r.s = infinite ? most : s;
+    r.inv = infinite ? 0.0f : y;
     return r;
 }
 // e4m3 of RN32(v * inv), four to a word.  |v * inv| <= 448 (1 + 2^-22), which rounds to 448.
@@ -60,6 +69,7 @@ __device__ __forceinline__ float across_rows_max(float v) {
 // converted to FP16, which holds every e4m3 value, and the 16-bit MFMAs sum their
 // products in FP32 (1.3e-8 of a random block's sum, measured).
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ i32x8 operand(u32x4 a, u32x4 b) {
@@ -73,7 +83,19 @@ __device__ __forceinline__ f16x8 widened(uint32_t a, uint32_t b) {
                         __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true)};
     return f16x8{v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
 }
+__device__ __forceinline__ f16x4 widened4(uint32_t a) {
+    const f16x2 v[2] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false),
+                        __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true)};
+    return f16x4{v[0][0], v[0][1], v[1][0], v[1][1]};
+}
 // 16 channels x 16 rows: a lane's 32 inputs of either operand.
+__device__ __forceinline__ f32x4 product16(const u32x4 (&w)[2], const f16x8 (&x)[4]) {
+    f32x4 p{};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        p = __builtin_amdgcn_mfma_f32_16x16x32_f16(widened(w[i / 2][i % 2 * 2], w[i / 2][i % 2 * 2 + 1]), x[i], p, 0, 0, 0);
+    return p;
+}
 template <bool EXACT>
 __device__ __forceinline__ f32x4 product16(const u32x4 (&w)[2], const u32x4 (&x)[2]) {
     f32x4 p{};
@@ -87,26 +109,6 @@ __device__ __forceinline__ f32x4 product16(const u32x4 (&w)[2], const u32x4 (&x)
     }
     return p;
 }
-// 32 channels x 32 rows: a lane's 32 inputs of either half.
-template <bool EXACT>
-__device__ __forceinline__ f32x16 product32(const u32x4 (&w)[2][2], const u32x4 (&x)[2][2]) {
-    f32x16 p{};
-    if constexpr (EXACT) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const u32x4 a = w[i / 4][i / 2 % 2], b = x[i / 4][i / 2 % 2];
-            p = __builtin_amdgcn_mfma_f32_32x32x16_f16(widened(a[i % 2 * 2], a[i % 2 * 2 + 1]),
-                                                       widened(b[i % 2 * 2], b[i % 2 * 2 + 1]), p, 0, 0, 0);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-            p = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(w[j][0], w[j][1]), operand(x[j][0], x[j][1]), p, 0, 0,
-                                                                0, 0, 0, 0);
-    }
-    return p;
-}
-
 // A value that is the same for a whole wave and that no kernel running meanwhile writes:
 // a scalar load, which does not count among the vector loads in flight.
 __device__ __forceinline__ float ld_uniform(const float* p) {

@@ -18,19 +18,22 @@ namespace {
 // One launch: every workgroup rounds the rows itself while its weights (16
 // channels, of both projections in a pair) are on their way.  Eight waves split
 // K in whole blocks; a wave rounds its own part of every row, so nothing is
-// shared before the sums meet in LDS.  M: rows, rounded up to a power of two.  U:
+// shared before the sums meet in LDS; what a wave writes for its own lanes is FP16, which
+// every e4m3 value is, and which the products take.  M: rows, rounded up to a power of two.  U:
 // blocks of a wave's part, all in flight at once.  LONG: parts of several
 // batches of U.
 template <class T, int M, int U, bool PAIR, bool LONG>
 __global__ __launch_bounds__(512) void fp8_decode_kernel(Fp8Args a, const T* x, uint64_t stride, uint32_t input) {
     constexpr int P = PAIR ? 2 : 1, kGroups = (U + 1) / 2;   // of two blocks
     constexpr bool kGiven = std::is_same_v<T, uint8_t>;
-    extern __shared__ __align__(16) unsigned char smem[];
+    // A wave's batch of rows as the products take it, the rows' starts spread over the banks.
+    constexpr int kBatch = M * U * 256 + (M - 1) / 2 * 128 + 16;
+    auto place = [](uint32_t row) { return row * (U * 256) + row % 2 * 16 + row / 2 * 128; };
+    __shared__ __align__(16) unsigned char smem[8][kBatch];
+    __shared__ float row_s[8][M][U];
     __shared__ f32x4 part[P][8][64];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t kbs = a.k_blocks, kb0 = kbs * w / 8, kb1 = kbs * (w + 1) / 8;
-    const uint32_t pitch = kbs * 128 + 64;   // bytes of a row in LDS: rows 16 banks apart
-    float* row_s = reinterpret_cast<float*>(smem + M * pitch);   // [M][kbs]
     const uint32_t c = blockIdx.x;           // 16 channels
     // blocks past the wave's part read zeros
     const auto gr = make_rsrc(a.w + uint64_t(PAIR ? c / 2 * 4 + c % 2 : c) * kbs * 2048, kb1 * 2048);
@@ -38,8 +41,8 @@ __global__ __launch_bounds__(512) void fp8_decode_kernel(Fp8Args a, const T* x, 
     const float* t[2] = {a.t + uint64_t(c / 8) * kbs, a.t + a.t_up + uint64_t(c / 8) * kbs};
     u32x4 f[P][U][2];
     const uint32_t m = lane & 15;
-    const unsigned char* xr = smem + (m < a.rows ? m : 0) * pitch + (lane >> 4) * 16;   // dead columns repeat row 0
-    const float* xs = row_s + (m < a.rows ? m : 0) * kbs;
+    const uint32_t of = m < a.rows ? m : 0;   // dead columns repeat row 0
+    const unsigned char* xr = smem[w] + place(of) + (lane >> 4) * 32;
     f32x4 acc[P] = {};
     for (uint32_t kb = kb0; kb < kb1; kb += U) {
         // The rows first: loads arrive in order.  A lane has four inputs of a group of
@@ -82,9 +85,10 @@ __global__ __launch_bounds__(512) void fp8_decode_kernel(Fp8Args a, const T* x, 
                     q = round4(v, b.inv);
                     s = b.s;
                 }
-                if (at < kb1) {   // the second block may be another wave's
-                    *reinterpret_cast<uint32_t*>(smem + r * pitch + at * 128 + (lane & 31) * 4) = q;
-                    if ((lane & 31) == 0) row_s[r * kbs + at] = s;
+                const int u = 2 * g + (lane >> 5);
+                if (U % 2 == 0 || u < U) {
+                    *reinterpret_cast<f16x4*>(smem[w] + place(r) + u * 256 + (lane & 31) * 8) = widened4(q);
+                    if ((lane & 31) == 0) row_s[w][r][u] = s;
                 }
             }
         // a wave reads what it wrote itself: its LDS operations are in order
@@ -94,18 +98,22 @@ __global__ __launch_bounds__(512) void fp8_decode_kernel(Fp8Args a, const T* x, 
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (kb + u >= kb1) break;
-            const u32x4 q[2] = {*reinterpret_cast<const u32x4*>(xr + (kb + u) * 128),
-                                *reinterpret_cast<const u32x4*>(xr + (kb + u) * 128 + 64)};
-            const float s = xs[kb + u];
+            f16x8 q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const f16x8*>(xr + u * 256 + i / 2 * 128 + i % 2 * 16);
+            const float s = row_s[w][of][u];
 #pragma unroll
             for (int p = 0; p < P; ++p) {
-                const f32x4 v = product16<true>(f[p][u], q);
+                const f32x4 v = product16(f[p][u], q);
                 const float st = s * ld_uniform(t[p] + kb + u);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[p][i] = __builtin_fmaf(v[i], st, acc[p][i]);
             }
         }
         if (!LONG) break;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // read before the next batch is written
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 #pragma unroll
     for (int p = 0; p < P; ++p) part[p][w][lane] = acc[p];
@@ -248,25 +256,24 @@ __global__ __launch_bounds__(512, S::kSimd) void fp8_split_kernel(Fp8Args a) {
 
 template <class T, bool PAIR>
 hipError_t decode(const Fp8Args& a, const OpRows& x, uint32_t input, hipStream_t stream) {
-    auto go = [&](auto kernel, uint32_t rows) {
-        const size_t lds = size_t(rows) * (a.k_blocks * 132 + 64);
-        hipLaunchKernelGGL(kernel, dim3((a.output + 15) / 16), dim3(512), lds, stream, a,
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((a.output + 15) / 16), dim3(512), 0, stream, a,
                            static_cast<const T*>(x.data), x.stride, input);
         return hipGetLastError();
     };
     // U: blocks of a wave, an eighth of all
     auto go_rows = [&](auto rows) {
         constexpr int M = decltype(rows)::value;
-        if (a.k_blocks <= 16) return go(fp8_decode_kernel<T, M, 2, PAIR, false>, M);
-        if (a.k_blocks <= 32) return go(fp8_decode_kernel<T, M, 4, PAIR, false>, M);
-        if (a.k_blocks <= 40) return go(fp8_decode_kernel<T, M, 5, PAIR, false>, M);
-        return go(fp8_decode_kernel<T, M, 4, PAIR, true>, M);
+        if (a.k_blocks <= 16) return go(fp8_decode_kernel<T, M, 2, PAIR, false>);
+        if (a.k_blocks <= 32) return go(fp8_decode_kernel<T, M, 4, PAIR, false>);
+        if (a.k_blocks <= 40) return go(fp8_decode_kernel<T, M, 5, PAIR, false>);
+        return go(fp8_decode_kernel<T, M, 4, PAIR, true>);
     };
     using std::integral_constant;
     if (a.rows <= 1) return go_rows(integral_constant<int, 1>{});
     if (a.rows <= 2) return go_rows(integral_constant<int, 2>{});
     if (a.rows <= 4) return go_rows(integral_constant<int, 4>{});
-    return a.k_blocks <= 16 ? go(fp8_decode_kernel<T, 8, 2, PAIR, false>, 8) : hipErrorInvalidValue;
+    return a.k_blocks <= 16 ? go(fp8_decode_kernel<T, 8, 2, PAIR, false>) : hipErrorInvalidValue;
 }
 
 template <class F>

@@ -25,7 +25,7 @@ Fp8Plan fp8_plan(uint64_t rows, uint32_t input, uint32_t output, bool pair, bool
         p.bytes += (rows * output * 4 + 255) & ~uint64_t(255);
     };
     const bool decode = rows <= 2 || (rows <= 4 && input <= 8192) || (rows <= 8 && input <= 2048);
-    if (decode && rows * (kbs * 132 + 64) <= kFp8DecodeLds) {
+    if (decode) {
         place_hidden();
         return p;
     }

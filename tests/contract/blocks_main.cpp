@@ -508,11 +508,7 @@ static void sizing() {
                     const stx::Fp8Plan p = stx::fp8_plan(rows, I, N, pair, exact, rounded);
                     const uint64_t kbs = stx::fp8_k_blocks(I);
                     if (p.core == stx::kFp8Decode) {
-                        // rows in LDS, rounded up to a power of two, beside 8 KiB of sums a projection
-                        uint64_t m = 1;
-                        while (m < rows) m *= 2;
-                        CHECK(rows <= 8 && m * (kbs * 132 + 64) + 16384 <= 65536);
-                        CHECK(rows <= 4 || kbs <= 16);
+                        CHECK(rows <= 2 || (rows <= 4 && I <= 8192) || (rows <= 8 && I <= 2048));
                         CHECK(p.bytes == (rounded ? (rows * N * 4 + 255) / 256 * 256 : 0) && !p.hidden_at);
                         continue;
                     }
