@@ -536,6 +536,19 @@ static void sizing() {
                         CHECK(spread * 512 < uint64_t(1) << 32);
                     }
         }
+    // no tile is there for nothing: every kind of layer takes each that it can
+    bool taken[2][2][10] = {};
+    for (int kind = 0; kind < 4; ++kind)
+        for (uint64_t rows : {1, 5, 9, 33, 65, 130, 257, 333, 513, 1500, 2048, 4096})
+            for (uint32_t I : {128, 130, 300, 500, 1000, 2048, 4096, 6933})
+                for (uint32_t N : {16, 17, 130, 300, 2307, 4100, 5125, 8192, 12288})
+                    taken[kind & 1][kind / 2][stx::fp8_plan(rows, I, N, kind & 1, kind & 2, false).core] = true;
+    for (int kind = 0; kind < 4; ++kind)
+        for (uint32_t core = 0; core < 10; ++core) {
+            const bool narrow = core == stx::kFp8Split16x16 || core == stx::kFp8Split16x32;
+            CHECK(taken[kind & 1][kind / 2][core] ==
+                  !((kind & 1 && narrow) || (kind & 2 && core == stx::kFp8Wide256x256)));
+        }
     for (uint64_t rows : {1ull, 4ull, 64ull, 511ull, 512ull, 100000ull})
         for (uint32_t vocab : {1u, 2048u, 8192u, 8193u, 129280u, 2147483647u})
             for (uint32_t type : {F32, BF16}) {
