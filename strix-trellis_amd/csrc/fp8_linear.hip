@@ -173,7 +173,8 @@ __global__ __launch_bounds__(512, S::kSimd) void fp8_split_kernel(Fp8Args a) {
     constexpr uint32_t kSpan = PAIR ? (TN + 3) / 4 * 4 : TN;
     const auto wr = make_rsrc(a.w + uint64_t(PAIR ? c0 / 2 * 4 : c0) * block_row, kSpan * block_row);
     const auto xr = make_rsrc(a.x + uint64_t(mt) * TM * block_row, TM * block_row);
-    const float* s = a.s + mt * 16 * TM + (lane & 15);
+    const auto sr = make_rsrc(a.s, kbs * a.s_pitch * 4);
+    const uint32_t s_at = (mt * 16 * TM + (lane & 15)) * 4;
     struct Operands {
         u32x4 f[U][TN][2], g[U][TM][2];
         float s[U][TM];
@@ -181,9 +182,10 @@ __global__ __launch_bounds__(512, S::kSimd) void fp8_split_kernel(Fp8Args a) {
     auto load = [&](Operands& o, uint32_t kb) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            // past the wave's part: out of range, zeros
+            // Past the wave's part: a batch that starts there is not multiplied; of one that ends there
+            // the rest is out of range, zeros (scales too: a block's may be infinite).
             const bool live = kb + u < kb1;
-            const uint32_t at = live ? kb + u : kb0, lane_at = lane * 16 + (live ? 0 : 0x80000000u);
+            const uint32_t at = live ? kb + u : kb0, past = live || u == 0 ? 0 : 0x80000000u, lane_at = lane * 16 + past;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -194,17 +196,20 @@ __global__ __launch_bounds__(512, S::kSimd) void fp8_split_kernel(Fp8Args a) {
                     o.g[u][k][j] = __builtin_amdgcn_raw_buffer_load_b128(xr, lane_at + j * 1024, x_at[k] + at * 2048, 0);
             }
 #pragma unroll
-            for (int k = 0; k < TM; ++k) o.s[u][k] = ld_global(s + uint64_t(at) * a.s_pitch + k * 16);
+            for (int k = 0; k < TM; ++k)
+                o.s[u][k] = __builtin_bit_cast(
+                    float, __builtin_amdgcn_raw_buffer_load_b32(sr, (s_at + past) + k * 64, at * a.s_pitch * 4, 0));
         }
     };
     f32x4 acc[TN][TM] = {};
     auto multiply = [&](const Operands& o, uint32_t kb) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint32_t at = kb + u < kb1 ? kb + u : kb0;   // past the part: operands of zeros
+            const bool live = u == 0 || kb + u < kb1;
+            const uint32_t at = live ? kb + u : kb0;
 #pragma unroll
             for (int i = 0; i < TN; ++i) {
-                const float by = ld_uniform(t[i] + at);
+                const float by_at = ld_uniform(t[i] + at), by = live ? by_at : 0.0f;
 #pragma unroll
                 for (int k = 0; k < TM; ++k) {
                     const f32x4 p = product16<EXACT>(o.f[u][i], o.g[u][k]);
@@ -218,7 +223,8 @@ __global__ __launch_bounds__(512, S::kSimd) void fp8_split_kernel(Fp8Args a) {
     };
     Operands o[2];
     load(o[0], kb0);
-    for (uint32_t kb = kb0; kb < kb1; kb += 2 * U) {
+    uint32_t kb = kb0;
+    for (; kb + U < kb1; kb += 2 * U) {
         // the next batch's loads stay ahead of this one's products
         load(o[1], kb + U);
         __builtin_amdgcn_sched_barrier(0);
@@ -229,6 +235,7 @@ __global__ __launch_bounds__(512, S::kSimd) void fp8_split_kernel(Fp8Args a) {
         multiply(o[1], kb + U);
         __builtin_amdgcn_sched_barrier(0);
     }
+    if (kb < kb1) multiply(o[0], kb);
     constexpr int kUnits = S::kUnits;
     auto place = [&](int row, int unit) { return row * (kUnits * 16) + ((unit ^ row) & (kUnits - 1)) * 16; };
 #pragma unroll

@@ -65,6 +65,45 @@ def test_bytes_stand_for_e4m3(ctx, rows):
     assert all(torch.equal(a, c) for a, c in zip(*outs))
 
 
+@pytest.mark.parametrize("rows,I,N", [(3, 1152, 300), (5, 2176, 130), (9, 1024, 17), (9, 7040, 130), (9, 4096, 4100), (33, 128, 4100),
+                                      (65, 128, 4100), (100, 1280, 640), (333, 1024, 2307), (700, 640, 130)])
+def test_rows_of_e4m3_wherever_they_lie(ctx, rows, I, N):
+    """Rows of whole blocks on 16-byte units are read in place, others are laid out first: the same bits, side by side or
+    inside wider rows."""
+    w, t, b = ref.weights(I, N, 30)
+    q, s = ref.round_rows(ref.rows_of(rows, I, 31))
+    for out in (torch.float32, torch.bfloat16):
+        plain = linear.run(ctx, w, t, b, q, out, s)
+        for left, right in ((16, 48), (1, 2), (0, 16)):
+            wide = torch.full((rows, left + I + right), 127, device=DEV, dtype=torch.uint8).view(ref.E4M3)   # NaN
+            wide[:, left:left + I] = q
+            assert torch.equal(plain, linear.run(ctx, w, t, b, wide[:, left:left + I], out, s)), (out, left)
+    z, mag = ref.product(q, s, w, t, b)
+    ref.check(linear.run(ctx, w, t, b, q, torch.float32, s), z, ref.unit(I) * mag, (rows, I, N))
+
+
+@pytest.mark.parametrize("rows", [2, 9, 40, 100, 300, 1100])
+@pytest.mark.parametrize("I", [128, 1100, 1152])
+def test_infinite_scales(ctx, rows, I):
+    """A block's infinite scale, of a row or of weights, gives infinities of its products' signs (and NaN where a product
+    is 0 or both signs meet), in every row and channel that has it."""
+    N = 300
+    w, t, _ = ref.weights(I, N, 40, bias=False)
+    q, s = ref.round_rows(ref.rows_of(rows, I, 41))
+    for last in (False, True):
+        s2, t2 = s.clone(), t.clone()
+        s2[0, -1 if last else 0] = INF
+        t2[1, -1 if last else 0] = INF
+        y = linear.run(ctx, w, t2, None, q, torch.float32, s2)
+        part = slice(I - I % 128 if I % 128 else I - 128, I) if last else slice(0, 128)
+        p = q[:, part].double() @ w[:, part].double().t().contiguous()
+        hit = torch.zeros(rows, N, device=DEV, dtype=torch.bool)
+        hit[0] = True
+        hit[:, 128:256] = True
+        assert bool((y[hit].double() == (p * INF)[hit]).logical_or(p[hit] == 0).all())
+        assert bool(torch.isfinite(y[~hit]).all())
+
+
 @pytest.mark.parametrize("rows", [2, 24, 280])
 def test_two_graphs_of_one_layer(ctx, rows):
     """Two captured steps on the same weights, on streams of their own and at the same time: each has its own
