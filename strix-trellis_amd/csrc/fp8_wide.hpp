@@ -136,7 +136,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp8_wide_kernel(Fp8Args a) {
     auto stage = [&](const u32x4 (&now)[TN][2], u32x4 (&next)[TN][2], uint32_t kb) {
         float t_now[kScales];
 #pragma unroll
-        for (int i = 0; i < kScales; ++i) t_now[i] = kb < kbs ? t_at[i] : 0.0f;
+        for (int i = 0; i < kScales; ++i) t_now[i] = t_at[i];
         load_w(next, kb + 1);
 #pragma unroll
         for (int k = 0; k < TM; ++k) {
@@ -191,10 +191,12 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp8_wide_kernel(Fp8Args a) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) read_x(k, 0, k);
     if constexpr (EXACT) widen(gh[0], g[0]);
-    for (uint32_t kb = 0; kb < kbs; kb += 2) {
+    uint32_t kb = 0;
+    for (; kb + 1 < kbs; kb += 2) {
         stage(f[0], f[1], kb);
-        stage(f[1], f[0], kb + 1);   // past the last stage: zeros
+        stage(f[1], f[0], kb + 1);
     }
+    if (kb < kbs) stage(f[0], f[1], kb);
 #pragma unroll
     for (int i = 0; i < TN; ++i) fold(TM - 1, i);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
