@@ -19,6 +19,10 @@
 // 16, .. batches the list is cut to the first `top` keys, the last of which is the new bound: about
 // 1.4 `top` tokens enter between two cuts, and the waves meet only there.  A list that
 // overflowed in between is filled again from memory, with a higher bound.
+//
+// 64 x 8 beams of 129280 BF16, 16 kept: the pass 37 us (3.2 TB/s of the rows it reads; its vector steps take half the cycles,
+// and two batches on their way for three took 3 us more), the join 5 us.  4 beams of 129280 F32: 5.5 and 5.2,
+// a chain of round trips each.
 #include "beam.hpp"
 #include "logprobs_device.hpp"
 
@@ -228,7 +232,8 @@ struct JoinArgs {
 // The beams' lists of keys, first keys first, are taken 1024 at a time (nearly always all of them at
 // once); what reaches a bound that `keep` of them reach enters a list in LDS, whose first `keep` are
 // found by counting who is ahead of whom.  The lists are sorted, so behind a round of which none
-// enters there is nothing.
+// enters there is nothing.  Keys dealt list by list to the waves would leave a wave with the lowest beam
+// alone, whose keys then bound nothing (22 us for 5 with eight beams).
 __global__ __launch_bounds__(kThreads) void beam_join_kernel(JoinArgs a) {
     constexpr uint32_t kRound = 2 * kThreads, kList = kRound + 2 * kMaxBeams;   // + kept ones and pad tokens
     __shared__ Candidate list[kList];
@@ -429,6 +434,7 @@ __device__ __forceinline__ void move(const uint8_t* from, uint64_t from_row, uin
 
 // A thread moves one unit of N bytes of every beam of a prompt: it reads all of them
 // before it writes one, so that source and target may be one.  B: beams at most.
+// Bytes: half of 64 rows' 8 MiB in place 92 us, 5.3 TB/s read and written.
 template <int B, int N, bool IN_PLACE>
 __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
     const uint64_t piece = a.piece + blockIdx.y, prompt = a.prompt + blockIdx.z;
