@@ -187,3 +187,39 @@ def test_falling_candidates_of_many_beams(ctx):
     """64 beams x 8 splits x 64 tokens in full order: more candidates than one round of the join takes."""
     x, scores, _ = beam.inputs(1, 64, 66000, torch.float32, 10)
     beam.check(ctx, x, scores * 0, None, 64, 64)
+
+
+def test_device_arrays_without_torch_tensors(ctx):
+    """A step on the library's own arrays, e4m3 as bytes, against the same step on tensors."""
+    import numpy as np
+    from strix_trellis import device
+    rng = np.random.default_rng(6)
+    rows, beams, I, N, V = 6, 3, 200, 260, 900
+    gate, up, head = (rng.standard_normal(s, dtype=np.float32) * 0.1 for s in ((N, I), (N, I), (V, N)))
+    x, scores = rng.standard_normal((rows, I), dtype=np.float32), -rng.random(rows, dtype=np.float32)
+    cache = rng.integers(0, 255, (2, rows, 3, 50), dtype=np.uint8)
+
+    def step(put, empty, stream):
+        pair = runtime.Fp8Weights(ctx, put(gate), None, up=put(up), stream=stream)
+        down = runtime.Fp8Weights(ctx, put(head), None, stream=stream)
+        h, hs, y = empty((rows, N), np.uint8), empty((rows, ref.blocks(N)), np.float32), empty((rows, V), np.float32)
+        out = [empty((rows // beams, beams), t) for t in (np.float32, np.int32, np.int32)]
+        states = put(cache)
+        runtime.fp8_gated(pair, put(x), h, y_scales=hs, stream=stream)
+        runtime.fp8_linear(down, h, y, x_scales=hs, stream=stream)
+        runtime.beam_select(ctx, y, put(scores), *out, beams, stream=stream)
+        runtime.beam_reorder(ctx, out[1], states, stream=stream)
+        (stream or torch.cuda).synchronize()
+        result = [a.numpy() if isinstance(a, device.DeviceArray) else a.cpu().numpy() for a in (h, hs, y, *out, states)]
+        pair.destroy()
+        down.destroy()
+        return result
+
+    own = step(device.DeviceArray.from_numpy, device.DeviceArray.empty, device.Stream(0))
+    tensors = step(lambda a: torch.from_numpy(a).to(DEV),
+                   lambda s, t: torch.zeros(s, device=DEV, dtype=getattr(torch, np.dtype(t).name)), None)
+    assert all(np.array_equal(a, b) for a, b in zip(own, tensors))
+    parents = own[4]
+    want = cache.reshape(2, rows // beams, beams, 3, 50)
+    want = np.stack([want[:, p, parents[p]] for p in range(rows // beams)], 1).reshape(cache.shape)
+    assert np.array_equal(own[6], want)
