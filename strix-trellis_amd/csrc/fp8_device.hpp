@@ -64,8 +64,8 @@ __device__ __forceinline__ float across_rows_max(float v) {
 // The 8-bit MFMAs (f8f6f4, at twice the rate of the 16-bit ones) align the products of eight
 // neighbouring inputs of a lane to the largest of them and drop what lies below 2^-13 of it:
 // 1.25e-5 of a random block's sum in the 2-norm, measured, where FP32 sums have 1e-7.
-// That is far below a 16-bit output's half step (2^-12 of the value for F16, 2^-9 for BF16) or e4m3's
-// (2^-4), and those outputs take them.  F32 outputs do not: their operands are
+// That is far below a 16-bit output's half step (2^-12 of the value for F16, 2^-9 for BF16), and those
+// outputs take them.  F32 outputs do not, nor e4m3 ones, which come with F32 scales: their operands are
 // converted to FP16, which holds every e4m3 value, and the 16-bit MFMAs sum their
 // products in FP32 (1.3e-8 of a random block's sum, measured).
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
