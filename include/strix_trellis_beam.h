@@ -27,7 +27,7 @@ extern "C" {
  * beam, then the lower token:
  *   next_scores[p][j] = c    parents[p][j] = b (0..beams-1)    tokens[p][j] = v
  * Candidates of -inf are none; places that are left have -inf, -1 and -1.  Values are compared as FP64
- * sums of FP32 statistics: beams whose values differ by less than about 1e-7 of log p may change
+ * sums of FP32 statistics: tokens of two beams whose values differ by less than about 1e-6 may change
  * places.  1 <= beams <= 64, 1 <= keep <= 64; rows a multiple of beams.  The workspace is 256-byte
  * aligned.  Outputs and workspace overlap nothing. */
 typedef struct strix_amd_beam_select_desc {

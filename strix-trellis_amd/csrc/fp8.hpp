@@ -13,8 +13,9 @@ constexpr uint32_t kE4M3 = 17;   // element type beside OpType's, with the ABI's
 // half are the inputs 16 piece + 0..15 of it, of row 16 rb + row % 16.  The order
 // of the inputs within a block is free in a product as long as both operands
 // share it, so the same bytes serve the 16x16x128 8-bit MFMA (a lane's 32 inputs are
-// its 16 of either half) and, widened, four 16x16x32 16-bit ones (8 of them each).  Inputs are padded to whole blocks with zeros; rows
-// to whole 32-row pairs, whose other rows hold anything.
+// its 16 of either half) and, widened, four 16x16x32 16-bit ones (8 of them each).
+// Inputs are padded to whole blocks with zeros; rows to whole 32-row pairs, whose
+// other rows hold anything.
 constexpr uint32_t fp8_k_blocks(uint64_t input) { return uint32_t((input + 127) / 128); }
 constexpr uint64_t fp8_row_blocks(uint64_t rows) { return (rows + 31) / 32 * 2; }
 constexpr uint64_t fp8_block_bytes(uint64_t rows, uint64_t input) {
