@@ -540,7 +540,7 @@ static void sizing() {
     bool taken[2][2][10] = {};
     for (int kind = 0; kind < 4; ++kind)
         for (uint64_t rows : {1, 5, 9, 33, 65, 130, 257, 333, 513, 1500, 2048, 4096})
-            for (uint32_t I : {128, 130, 300, 500, 1000, 2048, 4096, 6933})
+            for (uint32_t I : {128, 130, 300, 500, 1000, 2048, 4096, 6933, 8192})
                 for (uint32_t N : {16, 17, 130, 300, 2307, 4100, 5125, 8192, 12288})
                     taken[kind & 1][kind / 2][stx::fp8_plan(rows, I, N, kind & 1, kind & 2, false).core] = true;
     for (int kind = 0; kind < 4; ++kind)
