@@ -26,10 +26,11 @@ extern "C" {
  * hold a NaN, a +inf, or none above -inf.  Per prompt, the `keep` largest of these, equal ones by the lower
  * beam, then the lower token:
  *   next_scores[p][j] = c    parents[p][j] = b (0..beams-1)    tokens[p][j] = v
- * Candidates of -inf are none; places that are left have -inf, -1 and -1.  Values are compared as FP64
- * sums of FP32 statistics: tokens of two beams whose values differ by less than about 1e-6 may change
- * places.  1 <= beams <= 64, 1 <= keep <= 64; rows a multiple of beams.  The workspace is 256-byte
- * aligned.  Outputs and workspace overlap nothing. */
+ * Candidates of -inf are none, nor are those whose c is -inf in FP32 (masks of a type's lowest value with
+ * a scale above 1); places that are left have -inf, -1 and -1.  Values are compared as FP64
+ * sums of FP32 statistics: tokens of two beams whose values differ by less than about 1e-6, or by less
+ * than FP64 holds at their size, may change places.  1 <= beams <= 64, 1 <= keep <= 64; rows a multiple
+ * of beams.  The workspace is 256-byte aligned.  Outputs and workspace overlap nothing. */
 typedef struct strix_amd_beam_select_desc {
     uint32_t struct_size;
     uint32_t abi_version;

@@ -322,7 +322,8 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(JoinArgs a) {
 #pragma unroll
         for (int j = 0; j < 3; ++j) {
             const Candidate& k = mine[j];
-            if (k.c == -double(kInf) || float(k.c) < reach || (count == a.keep && !ahead_of(k, bound))) continue;
+            const float c = float(k.c);   // what leaves: a value below FP32's range is -inf, and no candidate
+            if (c == -kInf || c < reach || (count == a.keep && !ahead_of(k, bound))) continue;
             list[atomicAdd(&list_end, 1u)] = k;
         }
         __syncthreads();
