@@ -2,6 +2,7 @@
 // scale, fragments of blocks, and what becomes of the sums.
 #pragma once
 #include "fp8.hpp"
+#include "fp8_scale.hpp"
 #include "ops_device.hpp"
 
 namespace stx {
@@ -18,20 +19,14 @@ __device__ __forceinline__ float maximum(float a, float b) { return __builtin_el
 struct BlockScale {
     float s, inv;
 };
-// Both quotients are the rounded ones, in fewer steps than a division takes that has to
-// reach every pair of operands: q corrected once by its residual is RN32(most / 448) for every `most` of
-// which it counts; two Newton steps from a reciprocal that is off by at most a unit give
-// RN32(1 / s) (each proved by trying every mantissa).  Only an infinity needs a step of its own.
+// Both quotients are the rounded ones (fp8_scale.hpp), given that the instruction's reciprocal is off by at
+// most a unit.  Only an infinity needs a step of its own.
 __device__ __forceinline__ BlockScale block_scale(float most) {
-    constexpr float kBy = 1.0f / 448.0f;
     BlockScale r;
     const bool infinite = most == __builtin_inff();
-    const float q = most * kBy, s = maximum(__builtin_fmaf(__builtin_fmaf(-448.0f, q, most), kBy, q), kLeastScale);
-    float y = __builtin_amdgcn_rcpf(s);
-    y = __builtin_fmaf(__builtin_fmaf(-s, y, 1.0f), y, y);
-    y = __builtin_fmaf(__builtin_fmaf(-s, y, 1.0f), y, y);
+    const float s = maximum(over_448(most), kLeastScale);
     r.s = infinite ? most : s;
-    r.inv = infinite ? 0.0f : y;
+    r.inv = infinite ? 0.0f : inverse_from(s, __builtin_amdgcn_rcpf(s));
     return r;
 }
 // e4m3 of RN32(v * inv), four to a word.  |v * inv| <= 448 (1 + 2^-22), which rounds to 448.
