@@ -16,16 +16,14 @@ constexpr Float over_448(Float x) {
 }
 
 // RN32(1 / s) of a normal s with a normal inverse, from a float y at most one unit from it: two Newton
-// steps, which end on it for every mantissa but one.  s = 2^k (2 - 2^-23), all bits set, has its
-// inverse 2^-(k + 1) (1 + 2^-24 + ..) a hair above the middle of two floats, and the steps may
-// end on the lower one, 2^-(k + 1), whose last bit is then set; the upper one has it set.
+// steps, the last one's residual a unit of its own higher.  Without that they end on it for every mantissa
+// but one: s = 2^k (2 - 2^-23) has its inverse 2^-(k + 1) (1 + 2^-24 + 2^-48 ..) a hair above the middle of two floats,
+// from the lower of which the residual, 2^-24, loses that hair and leads to the middle, which goes down.
 template <class Float>
 constexpr Float inverse_from(Float s, Float y) {
-    constexpr uint32_t kMantissa = 0x7FFFFF;
     y = __builtin_fmaf(__builtin_fmaf(-s, y, 1.0f), y, y);
-    y = __builtin_fmaf(__builtin_fmaf(-s, y, 1.0f), y, y);
-    const bool full = (__builtin_bit_cast(uint32_t, s) & kMantissa) == kMantissa;
-    return __builtin_bit_cast(Float, __builtin_bit_cast(uint32_t, y) | uint32_t(full));
+    const Float e = __builtin_fmaf(-s, y, 1.0f);
+    return __builtin_fmaf(__builtin_fmaf(__builtin_fabsf(e), 0x1.8p-24f, e), y, y);   // 0.75 to 1.5 units of e
 }
 
 }  // namespace stx
