@@ -263,8 +263,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp8_wide_kernel(Fp8Args a) {
         }
     } else {
         // Each token tile turns around in the wave's own part of LDS (16-byte unit u of row r
-        // at unit u ^ r), so that a store covers whole rows of it.  A wave's LDS operations
-        // are in order: no barrier.
+        // at unit u ^ r), so that a store covers whole rows of it.  No barrier.
         constexpr int kUnits = 4 * kTiles, kRowsAtOnce = 64 / kUnits;
         unsigned char* turn = smem + w * (16 * kUnits * 16);
         const uint32_t unit = lane % kUnits, sub = lane / kUnits, n = n0 + unit * 4;
@@ -275,6 +274,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp8_wide_kernel(Fp8Args a) {
 #pragma unroll
             for (int i = 0; i < kTiles; ++i)
                 *reinterpret_cast<f32x4*>(turn + place(lane & 15, i * 4 + quad)) = acc[k][i];
+            lanes_meet();
 #pragma unroll
             for (uint32_t row = sub; row < 16; row += kRowsAtOnce) {
                 const uint32_t m = m0 + k * 16 + row;
@@ -282,6 +282,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp8_wide_kernel(Fp8Args a) {
                 if (!PAIR) v += bias;
                 if (m < a.rows && n < a.output) emit(a, m, n, v, !PAIR);
             }
+            lanes_meet();   // read before the next tile is written
         }
     }
 }

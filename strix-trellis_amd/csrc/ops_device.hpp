@@ -122,6 +122,15 @@ __device__ __forceinline__ float wave_max(float v) {
     return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
+// Between a wave's accesses to LDS of which one lane's writes are another's reads.  The hardware
+// keeps a wave's LDS operations in order; this has the compiler keep them so too, which sees
+// each lane's own accesses only.  No instruction.
+__device__ __forceinline__ void lanes_meet() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // 1 / (1 + e^-g), from e^-|g|, which does not overflow: e^-g does below -88, where the
 // gate is not 0 yet (it is below -104).  e^x = 2^n 2^r with n the integer nearest x log2 e,
 // log2 e in two parts, and n bounded where 2^n is 0 already; infinities and NaN go
