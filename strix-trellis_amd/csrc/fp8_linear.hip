@@ -94,10 +94,7 @@ __global__ __launch_bounds__(512) void fp8_decode_kernel(Fp8Args a, const T* x, 
                     if ((lane & 31) == 0) row_s[w][r][u] = s;
                 }
             }
-        // a wave reads what it wrote itself: its LDS operations are in order
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        lanes_meet();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (kb + u >= kb1) break;
@@ -114,9 +111,7 @@ __global__ __launch_bounds__(512) void fp8_decode_kernel(Fp8Args a, const T* x, 
             }
         }
         if (!LONG) break;
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // read before the next batch is written
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        lanes_meet();   // read before the next batch is written
     }
 #pragma unroll
     for (int p = 0; p < P; ++p) part[p][w][lane] = acc[p];

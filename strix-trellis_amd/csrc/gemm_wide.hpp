@@ -37,6 +37,7 @@
 #include <type_traits>
 
 #include "gemm_kernel.hpp"
+#include "ops_device.hpp"
 
 namespace stx {
 
@@ -471,7 +472,7 @@ __global__ __launch_bounds__(512) void gemm_wide_kernel(GemmArgs a) {
     // (row-major, 16-byte unit u of row r at unit u ^ r, free of bank conflicts both
     // ways): afterwards lane l holds channels 4 (l % 32) .. + 3 of row 2 i +
     // l / 32, and a store instruction writes two whole 512-byte row segments.
-    // A wave's LDS operations are in order, so no barrier is needed.  Measured:
+    // No barrier is needed, only the wave's own order.  Measured:
     // 22,200 -> 13,600 cycles per tile (plane stores 10,800 -> 8,700); calls, same
     // bits, M = 512 on 5120^2 55.8 -> 54.7 us, M = 2048 on 4096 -> 12288 220 -> 212
     // us, M = 3000 on 1280 -> 16384 166 -> 154 us.
@@ -515,10 +516,12 @@ __global__ __launch_bounds__(512) void gemm_wide_kernel(GemmArgs a) {
         auto put_plane = [&](auto imc) {
             take(imc, v);
             turn_put(v);
+            lanes_meet();
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, turn_get(i)), prsrc,
                                                        row_off(decltype(imc)::value, i), 0, 0);
+            lanes_meet();   // read before the next block is written
         };
         put_plane(first);
         if constexpr (TM == 2) put_plane(last);
@@ -647,8 +650,10 @@ __global__ __launch_bounds__(512) void gemm_wide_kernel(GemmArgs a) {
     auto finish = [&](auto imc) {
         h128(imc, v);
         turn_put(v);
+        lanes_meet();
         if (use_beta) emit(imc, std::true_type{});
         else emit(imc, std::false_type{});
+        lanes_meet();   // read before the next block is written
     };
     finish(first);
     if constexpr (TM == 2) finish(last);

@@ -595,8 +595,8 @@ __global__ __launch_bounds__(256, 2) void int8_wide_kernel(Int8Args a) {
     // A lane holds four consecutive channels of 32 rows here and there; each 32-row
     // block of a wave turns around in the wave's own part of LDS (16-byte unit u
     // of row r at unit u ^ r), after which a store covers whole rows of the
-    // block (512 contiguous bytes of two rows at TN = 4).  A wave's LDS operations
-    // are in order: no barrier.  The row loop stays a loop: written out for every
+    // block (512 contiguous bytes of two rows at TN = 4).  No barrier, only
+    // the wave's own order.  The row loop stays a loop: written out for every
     // type and edge the epilogue took 95 KB of code, more than the instruction
     // cache holds.
     constexpr int kUnits = 8 * TN, kRowsAtOnce = 64 / kUnits, kTurn = 32 * kUnits * 16;
@@ -622,12 +622,14 @@ __global__ __launch_bounds__(256, 2) void int8_wide_kernel(Int8Args a) {
                 *reinterpret_cast<i32x4*>(turn + (lane & 31) * (kUnits * 16) +
                                           (((i * 8 + 2 * q + h) ^ lane) & (kUnits - 1)) * 16) =
                     i32x4{acc[i][k][4 * q], acc[i][k][4 * q + 1], acc[i][k][4 * q + 2], acc[i][k][4 * q + 3]};
+        lanes_meet();
 #pragma unroll 4
         for (uint32_t row = sub; row < 32; row += kRowsAtOnce) {
             const uint32_t m = m_wave + k * 32 + row;
             const i32x4 v = *reinterpret_cast<const i32x4*>(turn + row * (kUnits * 16) + ((unit ^ row) & (kUnits - 1)) * 16);
             if (m < a.rows && inside) emit(a, m, n, v, row_s[row], c);
         }
+        lanes_meet();   // read before the next block is written
     }
 }
 

@@ -18,6 +18,14 @@ template __global__ void fp8_wide_kernel<WideShape<8, 4, 2, 4, 1, false>, true, 
 template __global__ void fp8_wide_kernel<WideShape<4, 4, 2, 4, 1, true>, true, false>(Fp8Args);
 } }
 """
+INT8 = '#include "int8_linear.hip"\n'
+GEMM = """#include "gemm_wide.hpp"
+namespace stx {
+template __global__ void gemm_wide_kernel<4, 0, 256, false>(GemmArgs);
+template __global__ void gemm_wide_kernel<4, 0, 128, false>(GemmArgs);
+}
+"""
+BARRIER = re.compile(r"s_barrier|llvm\.amdgcn\.s\.barrier")
 
 
 def kernels(tmp_path, source, name):
@@ -58,7 +66,7 @@ def blocks_of(lines):
 def unordered(lines):
     """(LDS accesses behind the last barrier, those of them that follow the other kind without the wave's barrier)."""
     blocks = blocks_of(lines)
-    behind = [(label, i) for label, (body, _) in blocks.items() for i, line in enumerate(body) if "s_barrier" in line]
+    behind = [(label, i) for label, (body, _) in blocks.items() for i, line in enumerate(body) if BARRIER.search(line)]
     last, first = behind[-1]
     seen, todo, bad, count = {}, [(last, frozenset())], set(), set()
     while todo:
@@ -69,7 +77,7 @@ def unordered(lines):
         seen[label] = seen.get(label, frozenset()) | since
         since = set(seen[label])
         for line in blocks[label][0][start:]:
-            if "llvm.amdgcn.wave.barrier" in line or "s_barrier" in line:
+            if "llvm.amdgcn.wave.barrier" in line or BARRIER.search(line):
                 since.clear()
                 continue
             access = re.search(r"\b(store|load) .*ptr addrspace\(3\)", line)
@@ -84,7 +92,8 @@ def unordered(lines):
     return len(count), sorted(bad)
 
 
-@pytest.mark.parametrize("source,name,kinds", [(FP8, "fp8_wide_kernel", 3)], ids=["fp8_wide"])
+@pytest.mark.parametrize("source,name,kinds", [(FP8, "fp8_wide_kernel", 3), (INT8, "int8_wide_kernel", 2),
+                                               (GEMM, "gemm_wide_kernel", 2)], ids=["fp8_wide", "int8_wide", "gemm_wide"])
 def test_lanes_meet_in_order(tmp_path, source, name, kinds):
     found = kernels(tmp_path, source, name)
     assert len(found) == kinds, sorted(found)
