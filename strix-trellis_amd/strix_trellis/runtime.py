@@ -877,6 +877,18 @@ class TokenLogprobsPlan(_OpPlan):
 # ---------------------------------------------------------------------------
 
 
+def _block_scales(t, rows, width, name):
+    """strix_amd_buffer of scales float32 [rows, ceil(width / 128)], dimensions of one aside; None: absent.
+
+    The library counts bytes only, so that scales of as many or more elements in another order would pass."""
+    want = (rows, -(-width // 128))
+    buffer = op_buffer(t)
+    if t is not None and [int(n) for n in t.shape if n != 1] != [n for n in want if n != 1] and \
+            t.numel() >= want[0] * want[1]:   # fewer are the library's to refuse
+        raise ValueError(f"{name} must be [{want[0]}, {want[1]}]")
+    return buffer
+
+
 class Fp8Weights:
     """Weights of a layer in 8-bit floating point: `w` on the device, float8_e4m3fn [N, I] with `scales` float32
     [ceil(N / 128), ceil(I / 128)], or a float32, float16 or bfloat16 [N, I] that is rounded per 128 x 128 block.
@@ -886,8 +898,10 @@ class Fp8Weights:
     def __init__(self, ctx, w, scales=None, bias=None, up=None, up_scales=None, up_bias=None, stream=None):
         self.ctx, self.lib = ctx, ctx.lib
         self.output, self.input, self.pair = int(w.shape[0]), int(w.shape[1]), up is not None
-        d = abi.header(abi.Fp8WeightsDesc, weights=op_view(w, e4m3=True), scales=op_buffer(scales),
-                       bias=op_buffer(bias), up=op_view(up, e4m3=True), up_scales=op_buffer(up_scales),
+        d = abi.header(abi.Fp8WeightsDesc, weights=op_view(w, e4m3=True),
+                       scales=_block_scales(scales, -(-self.output // 128), self.input, "scales"),
+                       bias=op_buffer(bias), up=op_view(up, e4m3=True),
+                       up_scales=_block_scales(up_scales, -(-self.output // 128), self.input, "up_scales"),
                        up_bias=op_buffer(up_bias))
         h = C.c_void_p()
         abi.check(self.lib.strix_amd_fp8_weights_prepare(ctx.handle, C.byref(d), C.byref(stream_desc(stream)),
@@ -910,7 +924,8 @@ def _with_workspace(ctx, query, d, workspace, stream, like):
 
 def _fp8_linear_desc(weights, x, y, x_scales, alpha, beta):
     return abi.header(abi.Fp8LinearDesc, weights=weights.handle, input=op_view(x, e4m3=True),
-                      input_scales=op_buffer(x_scales), output=op_view(y), alpha=alpha, beta=beta)
+                      input_scales=_block_scales(x_scales, int(x.shape[0]), int(x.shape[1]), "x_scales"),
+                      output=op_view(y), alpha=alpha, beta=beta)
 
 
 def fp8_linear_workspace_bytes(weights, x, y, x_scales=None):
@@ -944,8 +959,10 @@ GATED_ACTIVATIONS = {"silu": 0, "gelu": 1}
 
 def _fp8_gated_desc(weights, x, y, x_scales, y_scales, activation):
     return abi.header(abi.Fp8GatedDesc, weights=weights.handle, input=op_view(x, e4m3=True),
-                      input_scales=op_buffer(x_scales), output=op_view(y, e4m3=True),
-                      output_scales=op_buffer(y_scales), activation=GATED_ACTIVATIONS[activation])
+                      input_scales=_block_scales(x_scales, int(x.shape[0]), int(x.shape[1]), "x_scales"),
+                      output=op_view(y, e4m3=True),
+                      output_scales=_block_scales(y_scales, int(y.shape[0]), int(y.shape[1]), "y_scales"),
+                      activation=GATED_ACTIVATIONS[activation])
 
 
 def fp8_gated_workspace_bytes(weights, x, y, x_scales=None, y_scales=None, activation="silu"):
