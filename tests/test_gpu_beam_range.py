@@ -1,4 +1,5 @@
-"""Selection of beams' continuations at the ends of FP32: candidates below its range.
+"""Selection of beams' continuations at the ends of FP32: candidates below its range, temperatures at both ends of what
+they may be, and joins that read their lists deep.
 
 Tolerance of a value, c = score + scale (x - m) - log(sum): the sum alone is held in FP32.  An exponential's argument has
 three half steps (the distance, scale log2 e, their product), 3 2^-24 z for an argument z = scale (m - x), which weighs
@@ -66,3 +67,53 @@ def test_scores_that_leave_fp32(ctx):
     v, p, t = beam.select(ctx, x[[0, 3]].contiguous(), scores[[0, 3]].contiguous(), None, 2, 6)
     assert p.tolist() == [[1, 0, -1, -1, -1, -1]] and t.tolist() == [[7, 7, -1, -1, -1, -1]]
     assert bool((v[0, 2:] == -INF).all())
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -16, 0.1, 1.0, 300.0, 2.0 ** 16])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_scales_with_their_tokens(ctx, scale, dtype):
+    """The permitted temperatures: each place's value, and its token, which has that value.  Within a beam the tokens are its
+    first ones in the order of the logits, whose distances the statistics do not touch."""
+    beams, keep, vocab = 3, 9, 10000
+    x, scores, finished = beam.inputs(2, beams, vocab, TYPES[dtype], 4)
+    got = beam.select(ctx, x, scores, finished, beams, keep, pad=5, scale=scale)
+    v = beam.reference(x, scores, finished, beams, keep, 5, scale)[0]
+    tol = 5e-6 * (1 + v.abs())
+    assert bool(((got[0].double() - v).abs() <= tol).logical_or(got[0].double() == v).all())
+    log_p = torch.log_softmax(x.double() * scale, 1)
+    order = torch.sort(x.float(), dim=1, descending=True, stable=True).indices
+    for prompt in range(2):
+        taken = [0] * beams
+        for j in range(keep):
+            value, b, token = float(got[0][prompt, j]), int(got[1][prompt, j]), int(got[2][prompt, j])
+            if b < 0:
+                assert token == -1 and value == -INF
+                continue
+            row = prompt * beams + b
+            if int(finished[row]):
+                assert token == 5 and taken[b] == 0 and value == float(scores[row])
+            else:
+                assert token == int(order[row, taken[b]]), (prompt, j)
+                assert abs(value - float(scores[row]) - float(log_p[row, token])) <= float(tol[prompt, j])
+            taken[b] += 1
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lists", [1, 3])
+def test_deep_lists_of_eight_splits(ctx, lists, dtype):
+    """64 beams of 129280 tokens in eight splits: 512 lists of 64 keys, of which a round of the join takes two each.  The
+    64 places go to a few lists, which have to be read to their ends."""
+    beams, vocab, keep = 64, 129280, 64
+    x, scores, _ = beam.inputs(1, beams, vocab, TYPES[dtype], 10)
+    scores = torch.full_like(scores, -1000.0)
+    for row, at, n in [(5, 40000, 64)] if lists == 1 else [(5, 40000, 30), (5, 80000, 30), (63, 129200, 30)]:
+        x[row, at:at + n] += 30.0
+        scores[row] = 0.0
+    (v, p, t), _ = beam.check(ctx, x, scores, None, beams, keep)
+    assert bool(((p == 5) | (p == 63)).all())
+
+
+def test_falling_candidates_of_eight_splits(ctx):
+    """512 lists in full order, no beam ahead of another."""
+    x, scores, _ = beam.inputs(1, 64, 129280, torch.float32, 10)
+    beam.check(ctx, x, scores * 0, None, 64, 64)
