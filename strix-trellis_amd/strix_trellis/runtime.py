@@ -1002,6 +1002,10 @@ def _beam_select_desc(logits, scores, next_scores, parents, tokens, beams, finis
     for t in (next_scores, parents, tokens):
         if t.dim() != 2 or int(t.shape[0]) != prompts or t.shape[1] != tokens.shape[1]:
             raise ValueError("next_scores, parents and tokens must be [prompts, keep]")
+    for t in (scores, finished):
+        shape = [] if t is None else [int(n) for n in t.shape if n != 1]
+        if beams > 1 and len(shape) > 1 and shape[-1] != beams:   # another order than the logits' rows
+            raise ValueError("scores and finished must be [prompts * beams]")
     return abi.header(abi.BeamSelectDesc, logits=op_view(logits), scores=op_buffer(scores),
                       finished=op_buffer(finished, "int32"), next_scores=op_buffer(next_scores),
                       parents=op_buffer(parents, "int32"), tokens=op_buffer(tokens, "int32"), beams=beams,
