@@ -60,7 +60,9 @@ strix_status strix_amd_beam_select_plan_create(strix_context context, const stri
  * (a cache [layers][rows][heads][length * size], of any capacity, is moved up to its length).  A parent
  * outside 0..beams-1 is the row itself.  `target` is `source` itself, with the same strides: rows that
  * are their own parents are then not touched; or memory that shares no byte with it.  Pieces
- * of the target do not overlap each other; strides of a dimension of one do not count.
+ * of the target do not overlap each other, and its dimensions lie within one another: with the strides in
+ * ascending order each is at least what the piece and the dimensions before it span (another layout is an
+ * unsupported format).  Strides of a dimension of one do not count.
  * 1 <= beams <= 64; source and target of any alignment. */
 typedef struct strix_amd_states {
     void *data;

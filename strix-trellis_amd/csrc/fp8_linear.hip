@@ -22,7 +22,7 @@ namespace {
 // every e4m3 value is, and which the products take.  M: rows, rounded up to a power of two.  U:
 // blocks of a wave's part, all in flight at once.  LONG: parts of several
 // batches of U.
-// Bound by the weights' bytes where there are many (5120 -> 129280, four BF16 rows: 114 us, 5.8 TB/s;
+// Bound by the weights' bytes where there are many (5120 -> 129280, four BF16 rows: 117 us, 5.7 TB/s;
 // of the vector units' time 70 % goes into rounding four rows in every workgroup), by the chain of
 // launch, row, rounding, products and sums where there are few (4096^2, one row: 4.9 us).
 template <class T, int M, int U, bool PAIR, bool LONG>

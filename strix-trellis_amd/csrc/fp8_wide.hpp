@@ -10,11 +10,12 @@ namespace {
 // The activations go through a ring of LDS stages of 128 inputs that the DMA fills
 // ahead; the weights' fragments, which lie in MFMA order, come straight from the
 // caches, a stage ahead in registers.
-// 2048 rows 4096 -> 12288 in 256 x 128: 107 us, 1.9 PFLOP/s; 8192^3 in 256 x 256: 490 us, 2.2 PFLOP/s (zeros, which
-// cost the clock less: 423).  A third of the waves' time goes into waiting for operands from the
+// Calls back to back, with the rounding of their BF16 rows: 2048 rows 4096 -> 12288 in 256 x 128 118 us, of which
+// about 111 are this kernel's, 1.9 PFLOP/s (in a kernel trace, which slows it, 113 at the least and 131 in the median); 8192^3 in
+// 256 x 256 496 us, 2.2 PFLOP/s (zeros, which cost the clock less: 423).  A third of the waves' time goes into waiting for operands from the
 // caches; the rest is shared by matrix steps and the vector steps beside them, of which an 8-bit MFMA hides
 // four (there are 4.9) and a 16-bit one one (3.4, with the widening).  EXACT, the gated pair of 2048 rows 4096 -> 2 x 12288:
-// 343 us, 1.2 PFLOP/s.
+// 352 us, of which about 346 are this kernel's, 1.2 PFLOP/s.
 template <int TM_, int TN_, int WM_, int WN_, int AHEAD_, bool EXACT_>
 struct WideShape {
     static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;
